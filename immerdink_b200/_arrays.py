@@ -63,7 +63,12 @@ _py.PyCapsule_GetName.argtypes = [C.py_object]
 _py.PyCapsule_GetName.restype = C.c_char_p
 
 
-def _from_dlpack(x, stream, device):
+def dlpack_view(x, stream, device):
+    """(ptr, shape, byte strides or None, (type code, bits, lanes), readonly, itemsize) of a DLPack
+    producer."""
+    if not hasattr(x, "__dlpack__"):
+        raise TypeError(f"{type(x).__name__} is not a CUDA array: it has neither "
+                        "__cuda_array_interface__ nor __dlpack__ (nothing is copied from the host)")
     kind, dev_id = (int(v) for v in x.__dlpack_device__())
     if kind not in (2, 13):  # kDLCUDA, kDLCUDAManaged
         raise TypeError(f"{type(x).__name__} is not in CUDA memory (DLPack device type {kind})")
@@ -88,18 +93,19 @@ def _from_dlpack(x, stream, device):
     shape = tuple(t.shape[i] for i in range(nd))
     item = t.bits * t.lanes // 8
     strides = None if not t.strides else tuple(t.strides[i] * item for i in range(nd))
-    f8 = t.code == 2 and t.bits == 64 and t.lanes == 1
-    return (t.data or 0) + t.byte_offset, shape, strides, f8, readonly, item
+    return (t.data or 0) + t.byte_offset, shape, strides, (t.code, t.bits, t.lanes), readonly, item
+
+
+def _from_dlpack(x, stream, device):
+    ptr, shape, strides, kind, readonly, item = dlpack_view(x, stream, device)
+    return ptr, shape, strides, kind == (2, 64, 1), readonly, item
 
 
 def view(x, stream=None, device=None):
     """(ptr, shape, byte strides or None, is_float64, readonly, itemsize) of a CUDA array."""
     cai = getattr(x, "__cuda_array_interface__", None)
     if cai is None:
-        if hasattr(x, "__dlpack__"):
-            return _from_dlpack(x, stream, device)
-        raise TypeError(f"{type(x).__name__} is not a CUDA array: it has neither "
-                        "__cuda_array_interface__ nor __dlpack__ (nothing is copied from the host)")
+        return _from_dlpack(x, stream, device)
     if cai.get("mask") is not None:
         raise TypeError("masked arrays are not supported")
     if _check_streams and stream is not None:

@@ -1,13 +1,15 @@
-"""In-tree build of the two shared libraries (no cmake):
+"""In-tree build of the shared libraries (no cmake):
 
     libimmerdink_host.so   CUDA-free host queries        (g++)
     libimmerdink.so        C ABI + sm_100a kernels       (nvcc -gencode arch=compute_100a,code=sm_100a)
     libimmerdink_hooks.so  the same objects + the imd_test_* / imd_prof_* entry points (tests, phase timing)
+    libimmerdink_linear.so C ABI + sm_100a kernels of the quantised linear layer (nvcc)
 
     python -m immerdink_b200.build [--force]
 
 The libraries land next to this file so that they travel with the source tree.
 """
+import concurrent.futures
 import os
 import subprocess
 import sys
@@ -19,6 +21,7 @@ INCLUDE = os.path.join(ROOT, "include")
 HOST_LIB = os.path.join(HERE, "libimmerdink_host.so")
 CUDA_LIB = os.path.join(HERE, "libimmerdink.so")
 HOOKS_LIB = os.path.join(HERE, "libimmerdink_hooks.so")
+LINEAR_LIB = os.path.join(HERE, "libimmerdink_linear.so")
 OBJ_DIR = os.path.join(HERE, "build")
 
 HOST_SOURCES = [os.path.join(CSRC, "host", f)
@@ -26,6 +29,8 @@ HOST_SOURCES = [os.path.join(CSRC, "host", f)
                           "perf_text.cpp")]
 CUDA_SOURCES = [os.path.join(CSRC, "cuda", f)
                 for f in ("api.cpp", "pipeline.cu", "gemm_tcgen05.cu")]
+
+LINEAR_SOURCES = [os.path.join(CSRC, "linear", f) for f in ("api.cpp", "norm.cu", "small.cu")]
 
 
 def _cxx():
@@ -66,6 +71,14 @@ def build_host(force=False):
     return HOST_LIB
 
 
+def _nvcc_command(verbose):
+    cmd = [_nvcc(), "-std=c++17", "-O3", "-lineinfo", "-gencode", "arch=compute_100a,code=sm_100a",
+           "-Xcompiler", "-fPIC,-fvisibility=hidden,-Wall", "-ccbin", _cxx(), "-I" + INCLUDE, "-I" + CSRC]
+    if verbose:
+        cmd[1:1] = ["-Xptxas", "-v"]
+    return cmd
+
+
 def build_cuda(force=False, verbose=False):
     """Kernel and ABI objects are compiled once; hooks.cpp twice (with and without IMD_HOOKS); the
     two libraries differ only in that object."""
@@ -75,10 +88,7 @@ def build_cuda(force=False, verbose=False):
                           for p in (CUDA_LIB, HOOKS_LIB))):
         return CUDA_LIB
     os.makedirs(OBJ_DIR, exist_ok=True)
-    common = [_nvcc(), "-std=c++17", "-O3", "-lineinfo", "-gencode", "arch=compute_100a,code=sm_100a",
-              "-Xcompiler", "-fPIC,-fvisibility=hidden,-Wall", "-ccbin", _cxx(), "-I" + INCLUDE, "-I" + CSRC]
-    if verbose:
-        common[1:1] = ["-Xptxas", "-v"]
+    common = _nvcc_command(verbose)
     objs, out = [], ""
     for src in CUDA_SOURCES:
         obj = os.path.join(OBJ_DIR, os.path.basename(src) + ".o")
@@ -99,9 +109,30 @@ def build_cuda(force=False, verbose=False):
     return CUDA_LIB
 
 
+def build_linear(force=False, verbose=False):
+    """libimmerdink_linear.so stands alone: it shares headers with the others but needs neither."""
+    src_time = _newest([os.path.join(CSRC, "linear"), os.path.join(CSRC, "cuda"), INCLUDE])
+    if not force and os.path.exists(LINEAR_LIB) and os.path.getmtime(LINEAR_LIB) >= src_time:
+        return LINEAR_LIB
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    jobs, objs = [], []
+    for src in LINEAR_SOURCES:
+        obj = os.path.join(OBJ_DIR, "linear_" + os.path.basename(src) + ".o")
+        objs.append(obj)
+        if force or not os.path.exists(obj) or os.path.getmtime(obj) < src_time:
+            jobs.append(_nvcc_command(verbose) + ["-c", src, "-o", obj])
+    with concurrent.futures.ThreadPoolExecutor(len(LINEAR_SOURCES)) as pool:
+        out = "".join(pool.map(_run, jobs))
+    out += _run([_nvcc(), "-shared", "-ccbin", _cxx(), *objs, "-o", LINEAR_LIB])
+    if verbose:
+        print(out)
+    return LINEAR_LIB
+
+
 def build_all(force=False, verbose=False):
     build_host(force)
     build_cuda(force, verbose)
+    build_linear(force, verbose)
 
 
 if __name__ == "__main__":
@@ -109,3 +140,4 @@ if __name__ == "__main__":
     print(HOST_LIB)
     print(CUDA_LIB)
     print(HOOKS_LIB)
+    print(LINEAR_LIB)

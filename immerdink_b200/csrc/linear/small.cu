@@ -1,0 +1,304 @@
+// Products with few rows of x: the weights' bytes are the cost, each is read once.
+//
+//   8 bits:  out[t, n] = xs[t] ws[n] sum_k x[t, k] w[n, k]
+//   4 bits:  out[t, n] = sum_g ws[n, g] sum_{k in g} x[t, k] (w[n, k] - z[n, g])
+//
+// A CTA owns 16 rows of w (one mma.sync row tile) and up to 8 NT rows of x; its eight warps take the
+// K chunks in turn and their partial sums are folded in a fixed order at the end. The order of k
+// inside a chunk is free as long as both operands use the same one: a lane takes the consecutive k of
+// its quarter of the chunk with one wide load per row, and whatever four (16-bit) or eight
+// (8-bit) of them a tensor instruction wants are already in its registers.
+//
+// 4-bit weights become exact 16-bit floats: a nibble or'ed into the mantissa of 128 (bf16) or 1024
+// (f16) is 128 + w or 1024 + w, and subtracting 128 + z or 1024 + z is exact. A shift by 4 i and one
+// lop3 give the nibbles i and i + 4 of a word as a pair, so the pairs of x are formed in that order
+// too. A quad of lanes covers one group, so a group's sum is one accumulator, scaled in 32 bits.
+// e4m3 values are exact in f16 and their products are summed in 32-bit floats by the f16 instruction.
+#include <cstdint>
+
+#include "types.cuh"
+
+namespace imd {
+namespace {
+
+constexpr int kWarps = 8;
+constexpr int kRowsPerTile = 16;
+
+__device__ __forceinline__ void mma_f16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_s8(int* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// `BYTES` bytes at p + at, zeros from `end` on. WIDE: p + at is aligned to BYTES and the whole piece
+// lies before `end` unless it starts there.
+template <int BYTES, bool WIDE>
+__device__ __forceinline__ void load_bytes(const uint8_t* p, int64_t at, int64_t end, uint32_t* v) {
+  if (WIDE && at + BYTES <= end) {
+    if (BYTES == 16) {
+      const uint4 t = *reinterpret_cast<const uint4*>(p + at);
+      v[0] = t.x, v[1 % (BYTES / 4)] = t.y, v[2 % (BYTES / 4)] = t.z, v[3 % (BYTES / 4)] = t.w;
+    } else if (BYTES == 8) {
+      const uint2 t = *reinterpret_cast<const uint2*>(p + at);
+      v[0] = t.x, v[1 % (BYTES / 4)] = t.y;
+    } else {
+      v[0] = *reinterpret_cast<const uint32_t*>(p + at);
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < BYTES / 4; ++i) {
+    uint32_t word = 0;
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+      if (at + 4 * i + b < end) word |= static_cast<uint32_t>(p[at + 4 * i + b]) << (8 * b);
+    v[i] = word;
+  }
+}
+// The same for 16-bit elements whose address is a multiple of 2 only.
+template <int WORDS, bool WIDE>
+__device__ __forceinline__ void load_halves(const uint16_t* p, int64_t at, int64_t end, uint32_t* v) {
+  if (WIDE && at + 2 * WORDS <= end) {
+#pragma unroll
+    for (int i = 0; i < WORDS; i += 4) {
+      const uint4 t = *reinterpret_cast<const uint4*>(p + at + 2 * i);
+      v[i] = t.x, v[i + 1] = t.y, v[i + 2] = t.z, v[i + 3] = t.w;
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < WORDS; ++i) {
+    uint32_t word = 0;
+    if (at + 2 * i < end) word = p[at + 2 * i];
+    if (at + 2 * i + 1 < end) word |= static_cast<uint32_t>(p[at + 2 * i + 1]) << 16;
+    v[i] = word;
+  }
+}
+
+__device__ __forceinline__ uint32_t sub_pair(uint32_t a, uint32_t b, __half) {
+  __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t sub_pair(uint32_t a, uint32_t b, __nv_bfloat16) {
+  __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  return *reinterpret_cast<uint32_t*>(&r);
+}
+__device__ __forceinline__ void mma_pair(float* d, const uint32_t* a, uint32_t b0, uint32_t b1, __half) {
+  mma_f16(d, a, b0, b1);
+}
+__device__ __forceinline__ void mma_pair(float* d, const uint32_t* a, uint32_t b0, uint32_t b1, __nv_bfloat16) {
+  mma_bf16(d, a, b0, b1);
+}
+
+__device__ __forceinline__ void store_out(const LinearArgs& p, int64_t t, int64_t n, float v) {
+  const int64_t i = t * p.out_stride + n;
+  if (p.out_type == IMD_TYPE_F32) static_cast<float*>(p.out)[i] = v;
+  else if (p.out_type == IMD_TYPE_F16) static_cast<__half*>(p.out)[i] = __float2half_rn(v);
+  else static_cast<__nv_bfloat16*>(p.out)[i] = __float2bfloat16_rn(v);
+}
+
+// Folds the warps' partial tiles in the order of the warps and hands each output to `write`.
+template <int NT, typename Acc, typename Write>
+__device__ __forceinline__ void fold(Acc (*acc)[4], const LinearArgs& p, int64_t n0, int64_t t0, Write write) {
+  __shared__ Acc part[kWarps][8 * NT][kRowsPerTile + 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      part[warp][8 * j + 2 * (lane & 3) + (i & 1)][(lane >> 2) + 8 * (i >> 1)] = acc[j][i];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 8 * NT * kRowsPerTile; i += 32 * kWarps) {
+    const int c = i / kRowsPerTile, r = i % kRowsPerTile;
+    Acc v = part[0][c][r];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) v += part[w][c][r];
+    if (t0 + c < p.rows && n0 + r < p.n) write(t0 + c, n0 + r, v);
+  }
+}
+
+template <typename X, int GROUP, int NT, bool WIDE>
+__global__ void __launch_bounds__(32 * kWarps) k_small_w4(const __grid_constant__ LinearArgs p) {
+  constexpr int kBytes = GROUP / 8;       // weights of one lane and row in one group
+  constexpr int kWords = kBytes / 4;
+  constexpr bool kHalf = sizeof(X) == 2 && __is_same(X, __half);
+  constexpr uint32_t kMagic = kHalf ? 0x64006400u : 0x43004300u;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t n0 = blockIdx.x * static_cast<int64_t>(kRowsPerTile), t0 = blockIdx.y * static_cast<int64_t>(8 * NT);
+  const int64_t row[2] = {min(n0 + (lane >> 2), p.n - 1), min(n0 + (lane >> 2) + 8, p.n - 1)};
+  const uint8_t* w[2] = {static_cast<const uint8_t*>(p.w) + row[0] * p.w_stride,
+                         static_cast<const uint8_t*>(p.w) + row[1] * p.w_stride};
+  const int64_t w_end = (p.k + 1) / 2;
+  const int64_t groups = (p.k + GROUP - 1) / GROUP;
+  float acc[NT][4] = {};
+  for (int64_t g = warp; g < groups; g += kWarps) {
+    const int64_t k0 = g * GROUP + (lane & 3) * (GROUP / 4);
+    uint32_t q[2][kWords], zero[2];
+    float scale[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      load_bytes<kBytes, WIDE>(w[h], k0 / 2, w_end, q[h]);
+      scale[h] = load_scale(p.scale4, p.scale_type, row[h] * p.scale_stride + g);
+      const uint32_t z = p.zeros == nullptr ? 8u : p.zeros[row[h] * p.zeros_stride + g] & 15u;
+      zero[h] = kMagic | z | (z << 16);
+    }
+    uint32_t x[NT][kWords][4];  // eight consecutive values of x for each word of weights
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const int64_t t = t0 + 8 * j + (lane >> 2);
+      if (t < p.rows) {
+        load_halves<4 * kWords, WIDE>(static_cast<const uint16_t*>(p.x) + t * p.x_stride, k0, p.k, &x[j][0][0]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4 * kWords; ++i) (&x[j][0][0])[i] = 0;
+      }
+    }
+    float sum[NT][4] = {};
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      uint32_t a[2][4];  // [row][pair]: pairs (0, 4), (1, 5), (2, 6), (3, 7) of the word
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+          a[h][b] = sub_pair(((q[h][i] >> (4 * b)) & 0x000F000Fu) | kMagic, zero[h], X());
+      const uint32_t a01[4] = {a[0][0], a[1][0], a[0][1], a[1][1]}, a23[4] = {a[0][2], a[1][2], a[0][3], a[1][3]};
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const uint32_t* v = x[j][i];
+        mma_pair(sum[j], a01, __byte_perm(v[0], v[2], 0x5410), __byte_perm(v[0], v[2], 0x7632), X());
+        mma_pair(sum[j], a23, __byte_perm(v[1], v[3], 0x5410), __byte_perm(v[1], v[3], 0x7632), X());
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[j][i] = fmaf(scale[i >> 1], sum[j][i], acc[j][i]);
+  }
+  fold<NT, float>(acc, p, n0, t0, [&](int64_t t, int64_t n, float v) { store_out(p, t, n, v); });
+}
+
+// 16 e4m3 values (4 words) as f16 pairs.
+__device__ __forceinline__ void widen(const uint32_t* q, uint32_t (*h)[2]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(q[i] >> (16 * b)), __NV_E4M3);
+      h[i][b] = static_cast<uint32_t>(r.x) | (static_cast<uint32_t>(r.y) << 16);
+    }
+}
+
+template <bool I8, int NT, bool WIDE>
+__global__ void __launch_bounds__(32 * kWarps) k_small_8(const __grid_constant__ LinearArgs p) {
+  using Acc = typename std::conditional<I8, int, float>::type;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t n0 = blockIdx.x * static_cast<int64_t>(kRowsPerTile), t0 = blockIdx.y * static_cast<int64_t>(8 * NT);
+  const uint8_t* w[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    w[h] = static_cast<const uint8_t*>(p.w) + min(n0 + (lane >> 2) + 8 * h, p.n - 1) * p.w_stride;
+  Acc acc[NT][4] = {};
+  for (int64_t c = warp; c * 64 < p.k; c += kWarps) {
+    const int64_t k0 = c * 64 + (lane & 3) * 16;
+    uint32_t q[2][4], x[NT][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) load_bytes<16, WIDE>(w[h], k0, p.k, q[h]);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const int64_t t = t0 + 8 * j + (lane >> 2);
+      if (t < p.rows) {
+        load_bytes<16, WIDE>(static_cast<const uint8_t*>(p.x) + t * p.x_stride, k0, p.k, x[j]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[j][i] = 0;
+      }
+    }
+    if constexpr (I8) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t a[4] = {q[0][2 * i], q[1][2 * i], q[0][2 * i + 1], q[1][2 * i + 1]};
+#pragma unroll
+        for (int j = 0; j < NT; ++j) mma_s8(acc[j], a, x[j][2 * i], x[j][2 * i + 1]);
+      }
+    } else {
+      uint32_t wide[2][4][2], wx[NT][4][2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) widen(q[h], wide[h]);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) widen(x[j], wx[j]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t a[4] = {wide[0][i][0], wide[1][i][0], wide[0][i][1], wide[1][i][1]};
+#pragma unroll
+        for (int j = 0; j < NT; ++j) mma_f16(acc[j], a, wx[j][i][0], wx[j][i][1]);
+      }
+    }
+  }
+  fold<NT, Acc>(acc, p, n0, t0, [&](int64_t t, int64_t n, Acc v) {
+    store_out(p, t, n, static_cast<float>(v) * p.x_scale[t] * p.w_scale8[n]);
+  });
+}
+
+bool rows_aligned(const void* p, int64_t stride_bytes, int64_t rows, int unit) {
+  return reinterpret_cast<uintptr_t>(p) % unit == 0 && (rows <= 1 || stride_bytes % unit == 0);
+}
+
+template <int NT, bool WIDE>
+void launch(const LinearArgs& a, dim3 grid, cudaStream_t stream) {
+  constexpr int threads = 32 * kWarps;
+  if (a.kind == WeightKind::kI8) {
+    k_small_8<true, NT, WIDE><<<grid, threads, 0, stream>>>(a);
+  } else if (a.kind == WeightKind::kE4M3) {
+    k_small_8<false, NT, WIDE><<<grid, threads, 0, stream>>>(a);
+  } else if (a.x_type == IMD_TYPE_F16) {
+    if (a.group == 128) k_small_w4<__half, 128, NT, WIDE><<<grid, threads, 0, stream>>>(a);
+    else if (a.group == 64) k_small_w4<__half, 64, NT, WIDE><<<grid, threads, 0, stream>>>(a);
+    else k_small_w4<__half, 32, NT, WIDE><<<grid, threads, 0, stream>>>(a);
+  } else {
+    if (a.group == 128) k_small_w4<__nv_bfloat16, 128, NT, WIDE><<<grid, threads, 0, stream>>>(a);
+    else if (a.group == 64) k_small_w4<__nv_bfloat16, 64, NT, WIDE><<<grid, threads, 0, stream>>>(a);
+    else k_small_w4<__nv_bfloat16, 32, NT, WIDE><<<grid, threads, 0, stream>>>(a);
+  }
+}
+
+}  // namespace
+
+imd_status_t linear_small_launch(const LinearArgs& a, cudaStream_t stream) {
+  const int x_size = a.kind == WeightKind::kU4 ? 2 : 1;
+  const int w_unit = a.kind == WeightKind::kU4 ? a.group / 8 : 16;
+  const bool wide = rows_aligned(a.x, a.x_stride * x_size, a.rows, 16) && rows_aligned(a.w, a.w_stride, a.n, w_unit);
+  const int nt = a.rows <= 8 ? 1 : a.rows <= 16 ? 2 : 4;
+  const int64_t tiles = (a.rows + 8 * nt - 1) / (8 * nt);
+  LinearArgs part = a;
+  for (int64_t t = 0; t < tiles; t += 65535) {  // the grid's second extent
+    const int64_t t0 = t * 8 * nt, count = tiles - t < 65535 ? tiles - t : 65535;
+    part.rows = a.rows - t0;
+    part.x = static_cast<const uint8_t*>(a.x) + t0 * a.x_stride * x_size;
+    if (a.x_scale != nullptr) part.x_scale = a.x_scale + t0;
+    part.out = static_cast<uint8_t*>(a.out) + t0 * a.out_stride * (a.out_type == IMD_TYPE_F32 ? 4 : 2);
+    const dim3 grid(static_cast<unsigned int>((a.n + kRowsPerTile - 1) / kRowsPerTile), static_cast<unsigned int>(count));
+    if (nt == 1) wide ? launch<1, true>(part, grid, stream) : launch<1, false>(part, grid, stream);
+    else if (nt == 2) wide ? launch<2, true>(part, grid, stream) : launch<2, false>(part, grid, stream);
+    else wide ? launch<4, true>(part, grid, stream) : launch<4, false>(part, grid, stream);
+  }
+  return cudaGetLastError() == cudaSuccess ? IMD_STATUS_SUCCESS : IMD_STATUS_CUDA_ERROR;
+}
+
+}  // namespace imd
