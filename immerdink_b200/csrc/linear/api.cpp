@@ -3,6 +3,7 @@
 #include <cmath>
 #include <cstdint>
 
+#include "dense.hpp"
 #include "linear.hpp"
 
 namespace {
@@ -109,7 +110,7 @@ imd_status_t imd_scaled_linear(int64_t rows, int64_t n, int64_t k, int32_t type,
   a.out = out, a.out_stride = out_stride;
   a.kind = type == IMD_TYPE_I8 ? imd::WeightKind::kI8 : imd::WeightKind::kE4M3;
   a.x_type = type, a.out_type = out_type;
-  return imd::linear_small_launch(a, stream);
+  return imd::dense8_takes(a) ? imd::dense8_launch(a, stream) : imd::linear_small_launch(a, stream);
 }
 
 imd_status_t imd_linear_w4(int64_t rows, int64_t n, int64_t k, int32_t group, int32_t x_type,

@@ -1,0 +1,19 @@
+// The tensor-core kernels' share of a device: what is looked up or set once per device.
+#pragma once
+#include "linear.hpp"
+
+namespace imd {
+
+struct DeviceInfo {
+  void* encode_tiled = nullptr;  // cuTensorMapEncodeTiled
+  unsigned int* error_word = nullptr;
+  int sms = 0;
+};
+// Of the current device; made on first use, nullptr where that fails (asked again at the next call).
+const DeviceInfo* device_info();
+
+bool dense8_setup();                       // kernel attributes on the current device
+bool dense8_takes(const LinearArgs& a);    // whether the tensor-core kernels can take this call
+imd_status_t dense8_launch(const LinearArgs& a, cudaStream_t stream);
+
+}  // namespace imd

@@ -1,0 +1,560 @@
+// 8-bit products with many rows on the tensor cores:
+//
+//   out[t, n] = xs[t] ws[n] sum_k x[t, k] w[n, k]         int8: exact int32 sums; e4m3: 32-bit float sums
+//
+// Bound by the tensor pipe once both operands have a few hundred rows, by the weights' bytes below.
+// Two kernels share the pipeline of the contraction's GEMM (TMA into a ring of 128-byte K blocks with the
+// 128-byte swizzle, one thread issuing tcgen05.mma, accumulators in tensor memory):
+//
+//   k_dense8_pair   CTA pairs, 256 rows of x by BN rows of w per tile, persistent, two accumulators so that
+//                   the epilogue of a tile runs under the main loop of the next
+//   k_dense8_swap   up to 256 rows of x: the weights are the M side (128 of their rows per CTA, whatever
+//                   the rows of x), all rows of x the N side, so no tensor work is spent on padding and the
+//                   weights pass through once. A cluster of up to 8 CTAs splits K where the row tiles alone
+//                   would not fill the GPU; the parts are added through distributed shared memory in the
+//                   order of the ranks, so results do not depend on timing and no workspace is needed.
+//
+// Every wait is bounded: one that gives up sets the device error word, the roles drain and the CTA ends.
+#include <cstdint>
+#include <type_traits>
+
+#include "cuda/sm100.cuh"
+#include "dense.hpp"
+#include "types.cuh"
+
+namespace imd {
+namespace {
+
+constexpr int kThreads = 192;       // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue
+constexpr int kTileM = 128;         // rows of one CTA's accumulator
+constexpr int kTileK = 128;         // bytes of K per pipeline stage = one swizzle row
+constexpr int kMmaK = 32;
+constexpr int kBytesM = kTileM * kTileK;
+constexpr int kCtrlBytes = 256;     // barriers, tensor-memory address, abort flag
+
+struct Params {
+  int32_t rows, n, k_blocks;
+  int32_t tiles_m, tiles_n, band_rows;  // pair kernel
+  int32_t cols, stages, tmem_cols;      // swap kernel: rows of x padded to 16, ring depth
+  const float *x_scale, *w_scale;
+  void* out;
+  int64_t out_stride;
+  int32_t out_type, out_wide;           // out_wide: 16-byte stores are aligned
+  unsigned int* error_word;
+};
+
+// Instruction descriptor: D s32 (2) with A = B = s8 (1), or D f32 (1) with A = B = e4m3 (0); both K-major.
+template <bool I8>
+__host__ __device__ constexpr uint32_t instr_desc(int m, int n) {
+  return ((I8 ? 2u : 1u) << 4) | ((I8 ? 1u : 0u) << 7) | ((I8 ? 1u : 0u) << 10) |
+         (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+template <bool I8, bool PAIR>
+__device__ __forceinline__ void mma8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+  const uint32_t acc = add ? 1u : 0u;
+#define IMD_MMA8(GROUP, KIND)                                                              \
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"                           \
+               "tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], %1, %2, %3, p;\n\t}" \
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)                              \
+               : "memory")
+  if constexpr (PAIR && I8) IMD_MMA8("2", "i8");
+  else if constexpr (PAIR) IMD_MMA8("2", "f8f6f4");
+  else if constexpr (I8) IMD_MMA8("1", "i8");
+  else IMD_MMA8("1", "f8f6f4");
+#undef IMD_MMA8
+}
+
+template <bool I8>
+__device__ __forceinline__ float acc_value(uint32_t v) {
+  return I8 ? static_cast<float>(static_cast<int32_t>(v)) : __uint_as_float(v);
+}
+
+__device__ __forceinline__ void store_one(const Params& p, int64_t i, float v) {
+  if (p.out_type == IMD_TYPE_F32) static_cast<float*>(p.out)[i] = v;
+  else if (p.out_type == IMD_TYPE_F16) static_cast<__half*>(p.out)[i] = __float2half_rn(v);
+  else static_cast<__nv_bfloat16*>(p.out)[i] = __float2bfloat16_rn(v);
+}
+template <typename T>
+__device__ __forceinline__ void store_wide(void* out, int64_t i, const float* v) {
+  constexpr int V = 16 / sizeof(T);
+#pragma unroll
+  for (int c = 0; c < 16; c += V) {
+    Pack<T, V> o;
+#pragma unroll
+    for (int j = 0; j < V; ++j) o.v[j] = from_float<T>(v[c + j]);
+    *reinterpret_cast<Pack<T, V>*>(static_cast<T*>(out) + i + c) = o;
+  }
+}
+
+// ---- many rows: CTA pairs ------------------------------------------------------------------------------
+// Signals as in the contraction's pair kernel: full[s] in the leader, armed with the bytes of both CTAs;
+// empty[s] and tfull[a] by commits that reach both CTAs; tempty[a] in the leader, eight epilogue warps.
+template <int BN>
+constexpr int kPairStageBytes = kBytesM + BN / 2 * kTileK;
+template <int BN>
+constexpr int kPairStages = BN == 256 ? 6 : 8;
+template <int BN>
+constexpr int kPairSmem = kPairStages<BN> * kPairStageBytes<BN> + 1024 + kCtrlBytes;
+
+__device__ __forceinline__ void pair_tile(const Params& p, int w, int* tm, int* tn) {
+  const int band = p.band_rows * p.tiles_n;
+  const int first = (w / band) * p.band_rows;
+  const int rows = min(p.tiles_m - first, p.band_rows);
+  const int r = w % band;
+  *tm = first + r % rows;
+  *tn = r / rows;
+}
+
+template <bool I8, int BN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+k_dense8_pair(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+              const __grid_constant__ Params p) {
+  constexpr int kStages = kPairStages<BN>, kStageBytes = kPairStageBytes<BN>;
+  constexpr uint32_t kDesc = instr_desc<I8>(256, BN);
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t tiles = (raw + 1023u) & ~1023u;
+  uint8_t* ctrl = smem_raw + (tiles - raw) + kStages * kStageBytes;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ctrl + 200);
+  volatile int* abort = reinterpret_cast<volatile int*>(ctrl + 208);
+  const uint32_t bar0 = smem_u32(ctrl);
+  auto full = [&](int s) { return bar0 + 8u * s; };
+  auto empty = [&](int s) { return bar0 + 8u * (kStages + s); };
+  auto tfull = [&](int a) { return bar0 + 8u * (2 * kStages + a); };
+  auto tempty = [&](int a) { return bar0 + 8u * (2 * kStages + 2 + a); };
+  const uint32_t drain = bar0 + 8u * (2 * kStages + 4);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const bool leader = rank == 0;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(tfull(a), 1);
+      mbar_init(tempty(a), 8);
+    }
+    mbar_init(drain, 1);
+    *abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(2 * BN)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  const int total = p.tiles_m * p.tiles_n;
+  const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+  const uint32_t peer_abort = map_to_cta(smem_u32(const_cast<int*>(abort)), rank ^ 1u);
+  auto tell_peer = [&]() { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(peer_abort), "r"(1u) : "memory"); };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0, issued = 0;
+      bool okay = true;
+      const uint64_t policy = l2_policy(0);
+      for (int w = first; w < total && okay; w += step) {
+        int tm, tn;
+        pair_tile(p, w, &tm, &tn);
+        for (int kb = 0; kb < p.k_blocks; ++kb) {
+          if (!mbar_wait(empty(stage), phase ^ 1u, abort)) {
+            okay = false;
+            tell_peer();
+            break;
+          }
+          const uint32_t leader_full = map_to_cta(full(stage), 0);
+          if (leader) mbar_expect_tx(full(stage), 2 * kStageBytes);
+          const uint32_t dst = tiles + stage * kStageBytes;
+          tma_load_3d_pair(dst, &map_x, leader_full, kb * kTileK, tm * 256 + static_cast<int>(rank) * 128, 0, policy);
+          tma_load_3d_pair(dst + kBytesM, &map_w, leader_full, kb * kTileK,
+                           tn * BN + static_cast<int>(rank) * (BN / 2), 0, policy);
+          issued |= 1u << stage;
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      if (!okay && leader) {  // copies still in flight get a bounded time to land before the pair ends
+        for (int s = 0; s < kStages; ++s)
+          if (issued & (1u << s))
+            for (uint32_t it = 0; it < (1u << 20); ++it)
+              if (mbar_try_wait(full(s), 0) || mbar_try_wait(full(s), 1)) break;
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && leader) {
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool okay = true;
+      for (int w = first; w < total && okay; w += step) {
+        if (!mbar_wait(tempty(acc), acc_phase ^ 1u, abort)) {
+          tell_peer();
+          break;
+        }
+        tc_fence_after();
+        for (int kb = 0; kb < p.k_blocks; ++kb) {
+          if (!mbar_wait(full(stage), phase, abort)) {
+            okay = false;
+            tell_peer();
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a = tiles + stage * kStageBytes, b = a + kBytesM;
+#pragma unroll
+          for (int i = 0; i < kTileK / kMmaK; ++i)
+            mma8<I8, true>(tmem_base + acc * BN, smem_desc(a + i * kMmaK), smem_desc(b + i * kMmaK), kDesc, (kb | i) != 0);
+          tc_commit_pair(empty(stage));
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!okay) break;
+        tc_commit_pair(tfull(acc));
+        acc ^= 1;
+        if (acc == 0) acc_phase ^= 1u;
+      }
+      tc_commit_pair(drain, 1);
+      for (uint32_t it = 0; it < kSpinLimit; ++it)
+        if (mbar_try_wait(drain, 0)) break;
+    }
+  } else {
+    const int quarter = warp & 3;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    for (int w = first; w < total; w += step) {
+      int tm, tn;
+      pair_tile(p, w, &tm, &tn);
+      if (!mbar_wait(tfull(acc), acc_phase, abort)) {
+        if (lane == 0) tell_peer();
+        break;
+      }
+      tc_fence_after();
+      const int row = tm * 256 + static_cast<int>(rank) * 128 + quarter * 32 + lane;
+      const float xs = row < p.rows ? p.x_scale[row] : 0.0f;
+      const int64_t base = static_cast<int64_t>(row) * p.out_stride;
+      const uint32_t taddr = tmem_base + acc * BN + (static_cast<uint32_t>(quarter * 32) << 16);
+#pragma unroll 1
+      for (int cc = 0; cc < BN; cc += 32) {
+        const int col = tn * BN + cc;
+        if (col >= p.n) break;  // the same for the whole warp
+        uint32_t v[32];
+        tmem_load_32(taddr + cc, v);
+        if (row < p.rows) {
+#pragma unroll
+          for (int h = 0; h < 32; h += 16) {
+            float f[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              f[j] = col + h + j < p.n ? acc_value<I8>(v[h + j]) * xs * __ldg(p.w_scale + col + h + j) : 0.0f;
+            if (p.out_wide && col + h + 16 <= p.n) {
+              if (p.out_type == IMD_TYPE_F32) store_wide<float>(p.out, base + col + h, f);
+              else if (p.out_type == IMD_TYPE_F16) store_wide<__half>(p.out, base + col + h, f);
+              else store_wide<__nv_bfloat16>(p.out, base + col + h, f);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                if (col + h + j < p.n) store_one(p, base + col + h + j, f[j]);
+            }
+          }
+        }
+        __syncwarp();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(map_to_cta(tempty(acc), 0));
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1u;
+    }
+  }
+
+  tc_fence_before();
+  cluster_sync_all();  // no CTA leaves while its peer may still signal it or write its tensor memory
+  if (threadIdx.x == 0 && *abort) atomicOr(p.error_word, 1u);
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(2 * BN) : "memory");
+  }
+}
+
+// ---- up to 256 rows: weights on the M side ---------------------------------------------------------------
+constexpr int kSwapMaxStages = 12;
+constexpr int kFoldCols = 64;  // columns folded through shared memory at a time: 128 x 64 x 4 bytes
+
+__device__ __forceinline__ uint32_t load_cluster(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+template <bool I8>
+__global__ void __launch_bounds__(kThreads)
+k_dense8_swap(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
+              const __grid_constant__ Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t tiles = (raw + 1023u) & ~1023u;
+  const int stage_bytes = kBytesM + p.cols * kTileK;  // a multiple of 2048
+  uint8_t* ctrl = smem_raw + (tiles - raw) + p.stages * stage_bytes;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ctrl + 216);
+  volatile int* abort = reinterpret_cast<volatile int*>(ctrl + 224);
+  const uint32_t bar0 = smem_u32(ctrl);
+  auto full = [&](int s) { return bar0 + 8u * s; };
+  auto empty = [&](int s) { return bar0 + 8u * (kSwapMaxStages + s); };
+  const uint32_t done = bar0 + 8u * (2 * kSwapMaxStages);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int parts = gridDim.y, part = blockIdx.y;  // the cluster spans y: its rank is the part of K
+  const int kb0 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * part / parts);
+  const int kb1 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * (part + 1) / parts);
+  const int n0 = blockIdx.x * kTileM;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+    }
+    mbar_init(done, 1);
+    *abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(p.tmem_cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0, issued = 0;
+      bool okay = true;
+      const uint64_t policy_w = l2_policy(2), policy_x = l2_policy(1);  // weights stream through, x stays
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(empty(stage), phase ^ 1u, abort)) {
+          okay = false;
+          break;
+        }
+        mbar_expect_tx(full(stage), stage_bytes);
+        const uint32_t dst = tiles + stage * stage_bytes;
+        tma_load_3d(dst, &map_w, full(stage), kb * kTileK, n0, 0, policy_w);
+        tma_load_3d(dst + kBytesM, &map_x, full(stage), kb * kTileK, 0, 0, policy_x);
+        issued |= 1u << stage;
+        if (++stage == p.stages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (!okay) {
+        for (int s = 0; s < p.stages; ++s)
+          if (issued & (1u << s))
+            for (uint32_t it = 0; it < (1u << 20); ++it)
+              if (mbar_try_wait(full(s), 0) || mbar_try_wait(full(s), 1)) break;
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t idesc = instr_desc<I8>(kTileM, p.cols);
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(full(stage), phase, abort)) break;
+        tc_fence_after();
+        const uint32_t a = tiles + stage * stage_bytes, b = a + kBytesM;
+#pragma unroll
+        for (int i = 0; i < kTileK / kMmaK; ++i)
+          mma8<I8, false>(tmem_base, smem_desc(a + i * kMmaK), smem_desc(b + i * kMmaK), idesc, kb != kb0 || i != 0);
+        tc_commit(empty(stage));
+        if (++stage == p.stages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      tc_commit(done);  // arrives once every instruction issued above has retired
+    }
+  }
+  // every thread waits for the accumulator; the ring's memory is free for the fold after that
+  __syncwarp();
+  mbar_wait(done, 0, abort);
+  tc_fence_after();
+  __syncthreads();
+
+  const int quarter = warp & 3;
+  const int row = quarter * 32 + lane;                       // of the tile: a row of w
+  const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+  const float ws = n0 + row < p.n ? p.w_scale[n0 + row] : 0.0f;
+  if (parts == 1) {
+    if (warp >= 2) {
+#pragma unroll 1
+      for (int c = 0; c < p.cols; c += 32) {
+        uint32_t v[32];
+        tmem_load_32(taddr + c, v);
+        if (n0 + row < p.n) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (c + j < p.rows)
+              store_one(p, (c + j) * p.out_stride + n0 + row, acc_value<I8>(v[j]) * __ldg(p.x_scale + c + j) * ws);
+        }
+        __syncwarp();
+      }
+    }
+  } else {
+    for (int c0 = 0; c0 < p.cols; c0 += kFoldCols) {
+      const int width = min(kFoldCols, p.cols - c0);
+      if (warp >= 2) {
+        for (int c = 0; c < width; c += 32) {
+          uint32_t v[32];
+          tmem_load_32(taddr + c0 + c, v);
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (c + j < width)
+              asm volatile("st.shared.u32 [%0], %1;" ::"r"(tiles + ((c + j) * kTileM + row) * 4), "r"(v[j]) : "memory");
+        }
+      }
+      __syncwarp();
+      cluster_sync_all();
+      // part r adds columns r, r + parts, ...
+      if (warp >= 2 && n0 + row < p.n) {
+        for (int c = part; c < width; c += parts) {
+          if (c0 + c >= p.rows) break;
+          const uint32_t at = tiles + (c * kTileM + row) * 4;
+          uint32_t v = load_cluster(map_to_cta(at, 0));
+          for (int r = 1; r < parts; ++r) {
+            const uint32_t u = load_cluster(map_to_cta(at, r));
+            v = I8 ? v + u : __float_as_uint(__uint_as_float(v) + __uint_as_float(u));
+          }
+          store_one(p, (c0 + c) * p.out_stride + n0 + row, acc_value<I8>(v) * p.x_scale[c0 + c] * ws);
+        }
+      }
+      __syncwarp();
+      cluster_sync_all();  // the peers have read this CTA's columns
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && *abort) atomicOr(p.error_word, 1u);
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(p.tmem_cols) : "memory");
+  }
+}
+
+constexpr int kSwapSmem = 200 * 1024;
+
+bool encode_rows(const DeviceInfo& dev, CUtensorMap* map, const void* base, int64_t k, int64_t rows, int64_t stride, int box_rows) {
+  const int64_t pitch = rows > 1 ? stride : (k + 15) / 16 * 16;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rows), 1};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(pitch), static_cast<cuuint64_t>(pitch) * rows};
+  const cuuint32_t box[3] = {kTileK, static_cast<cuuint32_t>(box_rows), 1};
+  const cuuint32_t elem[3] = {1, 1, 1};
+  const EncodeTiled fn = reinterpret_cast<EncodeTiled>(dev.encode_tiled);
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, elem,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <bool I8, int BN>
+bool launch_pair(const LinearArgs& a, const DeviceInfo& dev, Params p, cudaStream_t stream) {
+  CUtensorMap mx, mw;
+  if (!encode_rows(dev, &mx, a.x, a.k, a.rows, a.x_stride, 128) ||
+      !encode_rows(dev, &mw, a.w, a.k, a.n, a.w_stride, BN / 2))
+    return false;
+  p.tiles_m = static_cast<int32_t>((a.rows + 255) / 256);
+  p.tiles_n = static_cast<int32_t>((a.n + BN - 1) / BN);
+  // rows of x walked together: about 32 MB of the 126 MB L2, as in the contraction's GEMM
+  const int64_t band = (INT64_C(32) << 20) / (256 * a.k);
+  p.band_rows = static_cast<int32_t>(band < 4 ? 4 : band);
+  if (p.band_rows > p.tiles_m) p.band_rows = p.tiles_m;
+  const int64_t total = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
+  if (total >= (INT64_C(1) << 31)) return false;
+  const int64_t pairs = total < dev.sms / 2 ? total : dev.sms / 2;
+  k_dense8_pair<I8, BN><<<static_cast<unsigned int>(2 * pairs), kThreads, kPairSmem<BN>, stream>>>(mx, mw, p);
+  return true;
+}
+
+template <bool I8>
+bool launch_swap(const LinearArgs& a, const DeviceInfo& dev, Params p, cudaStream_t stream) {
+  CUtensorMap mx, mw;
+  p.cols = static_cast<int32_t>((a.rows + 15) / 16 * 16);
+  p.tmem_cols = 32;
+  while (p.tmem_cols < p.cols) p.tmem_cols *= 2;
+  if (!encode_rows(dev, &mx, a.x, a.k, a.rows, a.x_stride, p.cols) ||
+      !encode_rows(dev, &mw, a.w, a.k, a.n, a.w_stride, kTileM))
+    return false;
+  const int64_t tiles = (a.n + kTileM - 1) / kTileM;
+  int parts = 1;  // CTAs that share a row tile: enough to occupy the SMs, at least two K blocks each
+  while (parts < 8 && tiles * parts * 2 <= dev.sms && p.k_blocks >= 4 * parts) parts *= 2;
+  const int stage_bytes = kBytesM + p.cols * kTileK;
+  p.stages = (kSwapSmem - 1024 - kCtrlBytes) / stage_bytes;
+  if (p.stages > kSwapMaxStages) p.stages = kSwapMaxStages;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned int>(tiles), static_cast<unsigned int>(parts));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = static_cast<size_t>(p.stages) * stage_bytes + 1024 + kCtrlBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {1, static_cast<unsigned int>(parts), 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, k_dense8_swap<I8>, mw, mx, p) == cudaSuccess;
+}
+
+template <bool I8>
+bool set_attributes() {
+  auto smem = [](const void* f, int bytes) {
+    return cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess;
+  };
+  return smem(reinterpret_cast<const void*>(k_dense8_pair<I8, 256>), kPairSmem<256>) &&
+         smem(reinterpret_cast<const void*>(k_dense8_pair<I8, 128>), kPairSmem<128>) &&
+         smem(reinterpret_cast<const void*>(k_dense8_swap<I8>), kSwapSmem);
+}
+
+template <bool I8>
+bool launch(const LinearArgs& a, const DeviceInfo& dev, const Params& p, cudaStream_t stream) {
+  if (a.rows <= 256) return launch_swap<I8>(a, dev, p, stream);
+  return launch_pair<I8, 256>(a, dev, p, stream);
+}
+
+}  // namespace
+
+bool dense8_setup() { return set_attributes<true>() && set_attributes<false>(); }
+
+// TMA wants 16-byte rows; a matrix whose rows overlap (a repeated row) stays with the small kernel.
+bool dense8_takes(const LinearArgs& a) {
+  auto rows_ok = [&](const void* p, int64_t rows, int64_t stride) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows == 1 || (stride % 16 == 0 && stride >= a.k));
+  };
+  return a.kind != WeightKind::kU4 && a.k > 0 && a.rows > 16 && rows_ok(a.x, a.rows, a.x_stride) && rows_ok(a.w, a.n, a.w_stride);
+}
+
+imd_status_t dense8_launch(const LinearArgs& a, cudaStream_t stream) {
+  const DeviceInfo* dev = device_info();
+  if (dev == nullptr) return IMD_STATUS_CUDA_ERROR;
+  Params p{};
+  p.rows = static_cast<int32_t>(a.rows), p.n = static_cast<int32_t>(a.n);
+  p.k_blocks = static_cast<int32_t>((a.k + kTileK - 1) / kTileK);
+  p.x_scale = a.x_scale, p.w_scale = a.w_scale8;
+  p.out = a.out, p.out_stride = a.out_stride, p.out_type = a.out_type;
+  const int unit = a.out_type == IMD_TYPE_F32 ? 4 : 8;
+  p.out_wide = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.out_stride % unit == 0;
+  p.error_word = dev->error_word;
+  const bool ok = a.kind == WeightKind::kI8 ? launch<true>(a, *dev, p, stream) : launch<false>(a, *dev, p, stream);
+  return cudaGetLastError() == cudaSuccess && ok ? IMD_STATUS_SUCCESS : IMD_STATUS_CUDA_ERROR;
+}
+
+}  // namespace imd

@@ -30,6 +30,7 @@ SIGNATURES = {
     "imd_norm_quantize": [_L, _L, _I, _P, _L, _P, _L, _I, _P, C.c_double, _P, _L, _I, _P, _L, _P, _P],
     "imd_scaled_linear": [_L, _L, _L, _I, _P, _L, _P, _L, _P, _P, _I, _P, _L, _P],
     "imd_linear_w4": [_L, _L, _L, _I, _I, _P, _L, _P, _L, _I, _P, _L, _P, _L, _I, _P, _L, _P],
+    "imd_linear_device_error": [C.POINTER(C.c_uint)],
 }
 
 
@@ -58,6 +59,14 @@ class Library:
                 break
             except OSError:
                 continue
+
+    def device_error(self):
+        """imd_linear_device_error: the sticky error word, read and cleared (synchronises)."""
+        v = C.c_uint(0)
+        st = self.lib.imd_linear_device_error(C.byref(v))
+        if st:
+            raise _error(st, "imd_linear_device_error")
+        return int(v.value)
 
     def current_device(self):
         """The current device's number; None where the runtime cannot be asked."""

@@ -84,6 +84,11 @@ IMD_API imd_status_t imd_linear_w4(int64_t rows, int64_t n, int64_t k, int32_t g
                                    int32_t out_type, void* out, int64_t out_stride,
                                    cudaStream_t stream);
 
+/* The sticky error word of this library on the current device, read into *word and cleared. Every wait
+ * inside its kernels is bounded; one that gives up sets bit 0 and the kernel ends with its output
+ * incomplete. Synchronises the device: a diagnostic, not part of a step. NULL -> INVALID_VALUE. */
+IMD_API imd_status_t imd_linear_device_error(unsigned int* word);
+
 #ifdef __cplusplus
 }
 #endif

@@ -28,6 +28,10 @@ def test_exports_are_the_header(lib):
     assert sorted(ln.split()[-1] for ln in out.splitlines() if " T " in ln and "imd_" in ln) == names
 
 
+def test_device_error_refuses(lib):
+    assert lib.imd_linear_device_error(None) == INVALID
+
+
 def test_missing_library_fails_loudly(monkeypatch):
     monkeypatch.setattr(os.path, "exists", lambda p: False)
     with pytest.raises(OSError, match="no CPU fallback"):

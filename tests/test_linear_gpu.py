@@ -18,6 +18,12 @@ BF16, F16, F32, I8, E4M3 = torch.bfloat16, torch.float16, torch.float32, torch.i
 U24 = 2.0 ** -24
 
 
+@pytest.fixture(autouse=True)
+def no_wait_gave_up():
+    yield
+    assert linear.load_library().device_error() == 0
+
+
 def half(t):
     return torch.finfo(t).eps / 2
 
