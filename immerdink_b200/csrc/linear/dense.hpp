@@ -12,8 +12,12 @@ struct DeviceInfo {
 // Of the current device; made on first use, nullptr where that fails (asked again at the next call).
 const DeviceInfo* device_info();
 
-bool dense8_setup();                       // kernel attributes on the current device
-bool dense8_takes(const LinearArgs& a);    // whether the tensor-core kernels can take this call
+// Kernel attributes on the current device; whether the tensor-core kernels take this call; the call.
+bool dense8_setup();
+bool dense8_takes(const LinearArgs& a);
 imd_status_t dense8_launch(const LinearArgs& a, cudaStream_t stream);
+bool dense4_setup();
+bool dense4_takes(const LinearArgs& a);
+imd_status_t dense4_launch(const LinearArgs& a, cudaStream_t stream);
 
 }  // namespace imd

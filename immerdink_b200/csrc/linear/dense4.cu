@@ -1,0 +1,385 @@
+// 4-bit weights with many rows of x on the tensor cores:
+//
+//   out[t, n] = sum_g ws[n, g] sum_{k in g} x[t, k] (w[n, k] - z[n, g])
+//
+// The weights are the M side (128 rows per CTA), up to 256 rows of x the N side. w - z is a small integer
+// and exact in x's 16-bit type, so the inner sum is an ordinary tcgen05.mma.kind::f16 with 32-bit
+// accumulators; the scale would not be exact there. So a group's sum is one accumulator of its own (two
+// in tensor memory, used in turn) and is added to registers as scale * sum while the next group is
+// multiplied: no weight is ever rounded, for one multiply-add per output and group. A row of w is one
+// lane of tensor memory, so its scale is one register.
+//
+// Warpgroups (512 threads, 128 registers each at launch, shared out again by setmaxnreg):
+//   0     warp 0 brings x by TMA (64 k = 128 bytes of a row, 128-byte swizzle), warp 1 issues the MMAs
+//   1     thread r turns row r of the weights' next 64 k into 16-bit floats in the swizzled layout
+//   2, 3  halves of the rows of x: out += scale * accumulator, then the stores
+// Bound by shared memory traffic for many rows (the operand tiles are written and read at about the port's rate),
+// by the unpacking's issue rate for few. A cluster of up to 8 CTAs splits K (whole groups) where the row tiles
+// alone would not fill the GPU; the parts are added through distributed shared memory in rank order.
+// Every wait is bounded, as in the 8-bit kernels.
+#include <cstdint>
+#include <type_traits>
+
+#include "cuda/sm100.cuh"
+#include "dense.hpp"
+#include "types.cuh"
+
+namespace imd {
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kRegsLaunch = 128;                                   // 65536 / kThreads
+constexpr int kRegsIssue = 40, kRegsUnpack = 104, kRegsSum = 176;  // per thread of warpgroup 0, 1, 2 and 3
+static_assert(kRegsIssue + kRegsUnpack + 2 * kRegsSum <= 4 * kRegsLaunch, "register shares above the launch's total");
+constexpr int kTileM = 128, kTileN = 256;
+constexpr int kBlockK = 64;                                        // k of one pipeline stage: 128 bytes a row
+constexpr int kBytesM = kTileM * 128;
+constexpr int kMaxStages = 8;
+constexpr int kCtrlBytes = 256;
+constexpr int kSmem = 200 * 1024;
+
+struct Params {
+  LinearArgs a;
+  int32_t units;                  // K in steps of max(group, 64)
+  int32_t tiles_t, cols, stages;  // row tiles of x; rows of x per tile, padded to 16
+  int32_t acc_cols;               // tensor-memory columns of one accumulator, a power of two
+  int32_t wide;                   // rows of w are 16-byte aligned
+  unsigned int* error_word;
+};
+
+template <typename X>
+__device__ __forceinline__ void mma16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(add ? 1u : 0u)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t load_cluster(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+template <typename X, int GROUP>
+__global__ void __launch_bounds__(kThreads, 1)
+k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ Params p) {
+  constexpr int kUnit = GROUP > kBlockK ? GROUP : kBlockK;       // k of one step of the split
+  constexpr int kBlocks = kUnit / kBlockK, kGroups = kUnit / GROUP;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t tiles = (raw + 1023u) & ~1023u;
+  const int stage_bytes = kBytesM + p.cols * 128;
+  uint8_t* ctrl = smem_raw + (tiles - raw) + p.stages * stage_bytes;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ctrl + 216);
+  volatile int* abort = reinterpret_cast<volatile int*>(ctrl + 224);
+  const uint32_t bar0 = smem_u32(ctrl);
+  auto full = [&](int s) { return bar0 + 8u * s; };
+  auto empty = [&](int s) { return bar0 + 8u * (kMaxStages + s); };
+  auto tfull = [&](int a) { return bar0 + 8u * (2 * kMaxStages + a); };
+  auto tempty = [&](int a) { return bar0 + 8u * (2 * kMaxStages + 2 + a); };
+  const uint32_t drain = bar0 + 8u * (2 * kMaxStages + 4);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wg = warp >> 2;
+  const int parts = gridDim.y, part = blockIdx.y;
+  const int u0 = static_cast<int>(static_cast<int64_t>(p.units) * part / parts);
+  const int u1 = static_cast<int>(static_cast<int64_t>(p.units) * (part + 1) / parts);
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x % p.tiles_t) * kTileN;
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x / p.tiles_t) * kTileM;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(full(s), 1 + 4);  // the TMA producer's arrival, and the four unpacking warps
+      mbar_init(empty(s), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(tfull(a), 1);
+      mbar_init(tempty(a), 8);
+    }
+    mbar_init(drain, 1);
+    *abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(2 * p.acc_cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (wg == 0) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
+    if (warp == 0 && lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0, issued = 0;
+      bool okay = true;
+      const uint64_t policy = l2_policy(1);  // x is read by every row tile of the weights
+      for (int kb = u0 * kBlocks; kb < u1 * kBlocks; ++kb) {
+        if (!mbar_wait(empty(stage), phase ^ 1u, abort)) {
+          okay = false;
+          break;
+        }
+        mbar_expect_tx(full(stage), p.cols * 128);
+        tma_load_3d(tiles + stage * stage_bytes + kBytesM, &map_x, full(stage), kb * kBlockK, static_cast<int>(t0), 0, policy);
+        issued |= 1u << stage;
+        if (++stage == p.stages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (!okay)  // copies still in flight get a bounded time to land
+        for (int s = 0; s < p.stages; ++s)
+          if (issued & (1u << s))
+            for (uint32_t it = 0; it < (1u << 20); ++it)
+              if (mbar_try_wait(full(s), 0) || mbar_try_wait(full(s), 1)) break;
+    } else if (warp == 1 && lane == 0) {
+      constexpr uint32_t kType = std::is_same<X, __nv_bfloat16>::value ? 1u : 0u;
+      const uint32_t idesc = (1u << 4) | (kType << 7) | (kType << 10) | (static_cast<uint32_t>(p.cols >> 3) << 17) |
+                             (static_cast<uint32_t>(kTileM >> 4) << 24);
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool okay = true;
+      for (int kb = u0 * kBlocks; kb < u1 * kBlocks && okay; ++kb) {
+        if (!mbar_wait(full(stage), phase, abort)) break;
+        tc_fence_after();
+        const uint32_t a = tiles + stage * stage_bytes, b = a + kBytesM;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // 16 k an instruction
+          const int at = (kb % kBlocks) * kBlockK + 16 * i;  // place in the unit
+          if (at % GROUP == 0) {
+            if (!mbar_wait(tempty(acc), acc_phase ^ 1u, abort)) {
+              okay = false;
+              break;
+            }
+            tc_fence_after();
+          }
+          mma16<X>(tmem_base + acc * p.acc_cols, smem_desc(a + 32 * i), smem_desc(b + 32 * i), idesc, at % GROUP != 0);
+          if ((at + 16) % GROUP == 0) {
+            tc_commit(tfull(acc));
+            acc ^= 1;
+            if (acc == 0) acc_phase ^= 1u;
+          }
+        }
+        if (okay) tc_commit(empty(stage));
+        if (++stage == p.stages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      tc_commit(drain);
+      for (uint32_t it = 0; it < kSpinLimit; ++it)
+        if (mbar_try_wait(drain, 0)) break;
+    }
+    __syncwarp();
+  } else if (wg == 1) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsUnpack));
+    const int r = threadIdx.x & 127;
+    const int64_t row = min(n0 + r, p.a.n - 1);
+    const uint8_t* w = static_cast<const uint8_t*>(p.a.w) + row * p.a.w_stride;
+    const uint8_t* zeros = p.a.zeros == nullptr ? nullptr : p.a.zeros + row * p.a.zeros_stride;
+    const int64_t end = (p.a.k + 1) / 2;
+    const int groups = static_cast<int>((p.a.k + GROUP - 1) / GROUP);
+    const Span span = span_of(p.a.w, p.a.n, p.a.w_stride, end);
+    auto fetch = [&](int kb, uint32_t* q) {
+      const int64_t at = static_cast<int64_t>(kb) * (kBlockK / 2);
+      if (p.wide) load_bytes<32, true>(w, at, end, span, q);
+      else load_bytes<32, false>(w, at, end, span, q);
+    };
+    uint32_t next[8];
+    const int kb1 = u1 * kBlocks;
+    int stage = 0;
+    uint32_t phase = 0;
+    if (u0 < u1) fetch(u0 * kBlocks, next);
+    for (int kb = u0 * kBlocks; kb < kb1; ++kb) {
+      uint32_t q[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) q[i] = next[i];
+      if (kb + 1 < kb1) fetch(kb + 1, next);
+      uint32_t zero[2];  // of the first and the second 32 k
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int g = (kb * kBlockK + 32 * h) / GROUP;
+        const uint32_t z = zeros == nullptr ? 8u : g < groups ? zeros[g] & 15u : 0u;
+        zero[h] = nibble_magic<X>() | z | (z << 16);
+      }
+      if (!mbar_wait(empty(stage), phase ^ 1u, abort)) break;
+      const uint32_t dst = tiles + stage * stage_bytes + r * 128;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {  // 16 bytes = 8 weights; the swizzle exchanges the pieces of a row by its number mod 8
+        uint32_t v[4];
+        nibble_pairs<X>(q[c], zero[c >> 2], v);
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst + ((c ^ (r & 7)) << 4)),
+                     "r"(__byte_perm(v[0], v[1], 0x5410)), "r"(__byte_perm(v[2], v[3], 0x5410)),
+                     "r"(__byte_perm(v[0], v[1], 0x7632)), "r"(__byte_perm(v[2], v[3], 0x7632))
+                     : "memory");
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the tensor core reads through the async proxy
+      __syncwarp();
+      if (lane == 0) mbar_arrive(full(stage));
+      if (++stage == p.stages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+    __syncwarp();
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSum));
+    const int quarter = warp & 3, row = quarter * 32 + lane;
+    const int64_t n = n0 + row, nc = min(n, p.a.n - 1);
+    const int half = (p.cols + 63) / 64 * 32;                     // columns of warpgroup 2
+    const int c0 = wg == 2 ? 0 : half, width = wg == 2 ? half : max(p.cols - half, 0);
+    const int groups = static_cast<int>((p.a.k + GROUP - 1) / GROUP);
+    const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + c0;
+    float sum[128];
+#pragma unroll
+    for (int j = 0; j < 128; ++j) sum[j] = 0.0f;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    const int g1 = u1 * kGroups;
+    auto scale_of = [&](int g) {
+      return g < groups ? load_scale(p.a.scale4, p.a.scale_type, nc * p.a.scale_stride + g) : 0.0f;
+    };
+    float next = scale_of(u0 * kGroups);
+    for (int g = u0 * kGroups; g < g1; ++g) {
+      const float scale = next;
+      if (g + 1 < g1) next = scale_of(g + 1);
+      if (!mbar_wait(tfull(acc), acc_phase, abort)) break;
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < 128; c += 32) {
+        if (c < width) {  // uniform
+          uint32_t v[32];
+          tmem_load_32(taddr + acc * p.acc_cols + c, v);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) sum[c + j] = fmaf(scale, __uint_as_float(v[j]), sum[c + j]);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(tempty(acc));
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1u;
+    }
+    __syncwarp();
+    if (parts == 1) {
+      if (n < p.a.n) {
+#pragma unroll
+        for (int j = 0; j < 128; ++j)
+          if (j < width && t0 + c0 + j < p.a.rows)
+            store_out(p.a.out, p.a.out_type, (t0 + c0 + j) * p.a.out_stride + n, sum[j]);
+      }
+    } else {
+      // the ring is free: the last group's accumulator was complete, so every operand had been read
+#pragma unroll
+      for (int j = 0; j < 128; ++j)
+        if (j < width)
+          asm volatile("st.shared.f32 [%0], %1;" ::"r"(tiles + ((c0 + j) * kTileM + row) * 4), "f"(sum[j]) : "memory");
+    }
+    __syncwarp();
+  }
+
+  if (parts > 1) {
+    cluster_sync_all();
+    if (wg >= 2) {
+      const int row = threadIdx.x & 127;
+      if (n0 + row < p.a.n) {
+        // part r adds columns r, r + parts, ...; the two warpgroups take them in turn
+        for (int c = part + parts * (wg - 2); c < p.cols; c += 2 * parts) {
+          if (t0 + c >= p.a.rows) break;
+          const uint32_t at = tiles + (c * kTileM + row) * 4;
+          float v = 0.0f;
+          for (int r = 0; r < parts; ++r) v += __uint_as_float(load_cluster(map_to_cta(at, r)));
+          store_out(p.a.out, p.a.out_type, (t0 + c) * p.a.out_stride + n0 + row, v);
+        }
+      }
+    }
+    __syncwarp();
+    cluster_sync_all();  // the peers have read this CTA's sums
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && *abort) atomicOr(p.error_word, 1u);
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(2 * p.acc_cols) : "memory");
+  }
+}
+
+using Kernel = void (*)(const CUtensorMap, const Params);
+template <typename X>
+Kernel kernel_of(int group) {
+  return group == 128 ? k_dense4<X, 128> : group == 64 ? k_dense4<X, 64> : k_dense4<X, 32>;
+}
+
+}  // namespace
+
+// The shares above are drawn from the registers of the launch, so a kernel compiled for fewer is refused.
+bool dense4_setup() {
+  for (int group : {32, 64, 128})
+    for (Kernel k : {kernel_of<__half>(group), kernel_of<__nv_bfloat16>(group)}) {
+      cudaFuncAttributes attr;
+      const void* f = reinterpret_cast<const void*>(k);
+      if (cudaFuncGetAttributes(&attr, f) != cudaSuccess || attr.numRegs < kRegsLaunch ||
+          cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
+        return false;
+    }
+  return true;
+}
+
+bool dense4_takes(const LinearArgs& a) {
+  return a.kind == WeightKind::kU4 && a.k > 0 && a.rows > 16 && reinterpret_cast<uintptr_t>(a.x) % 16 == 0 &&
+         a.x_stride % 8 == 0 && a.x_stride >= a.k;
+}
+
+imd_status_t dense4_launch(const LinearArgs& a, cudaStream_t stream) {
+  const DeviceInfo* dev = device_info();
+  if (dev == nullptr) return IMD_STATUS_CUDA_ERROR;
+  Params p{};
+  p.a = a;
+  const int unit = a.group > kBlockK ? a.group : kBlockK;
+  p.units = static_cast<int32_t>((a.k + unit - 1) / unit);
+  p.tiles_t = static_cast<int32_t>((a.rows + kTileN - 1) / kTileN);
+  p.cols = a.rows < kTileN ? static_cast<int32_t>((a.rows + 15) / 16 * 16) : kTileN;
+  p.acc_cols = 32;
+  while (p.acc_cols < p.cols) p.acc_cols *= 2;
+  p.wide = reinterpret_cast<uintptr_t>(a.w) % 16 == 0 && (a.n == 1 || a.w_stride % 16 == 0);
+  p.error_word = dev->error_word;
+  const int stage_bytes = kBytesM + p.cols * 128;
+  p.stages = (kSmem - 1024 - kCtrlBytes) / stage_bytes;
+  if (p.stages > kMaxStages) p.stages = kMaxStages;
+
+  CUtensorMap map;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(a.k), static_cast<cuuint64_t>(a.rows), 1};
+  const cuuint64_t pitch = static_cast<cuuint64_t>(a.x_stride) * 2;
+  const cuuint64_t strides[2] = {pitch, pitch * a.rows};
+  const cuuint32_t box[3] = {kBlockK, static_cast<cuuint32_t>(p.cols), 1};
+  const cuuint32_t elem[3] = {1, 1, 1};
+  if (reinterpret_cast<EncodeTiled>(dev->encode_tiled)(
+          &map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(a.x), dims, strides, box, elem,
+          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return IMD_STATUS_CUDA_ERROR;
+
+  const int64_t tiles = (a.n + kTileM - 1) / kTileM * p.tiles_t;
+  if (tiles >= (INT64_C(1) << 31)) return IMD_STATUS_NOT_SUPPORTED;
+  int parts = 1;  // CTAs that share a tile: enough to occupy the SMs, at least two steps of K each
+  while (parts < 8 && tiles * parts * 2 <= dev->sms && p.units >= 4 * parts) parts *= 2;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned int>(tiles), static_cast<unsigned int>(parts));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = static_cast<size_t>(p.stages) * stage_bytes + 1024 + kCtrlBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {1, static_cast<unsigned int>(parts), 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const Kernel k = a.x_type == IMD_TYPE_F16 ? kernel_of<__half>(a.group) : kernel_of<__nv_bfloat16>(a.group);
+  const bool ok = cudaLaunchKernelEx(&cfg, k, map, p) == cudaSuccess;
+  return cudaGetLastError() == cudaSuccess && ok ? IMD_STATUS_SUCCESS : IMD_STATUS_CUDA_ERROR;
+}
+
+}  // namespace imd

@@ -69,11 +69,6 @@ __device__ __forceinline__ float acc_value(uint32_t v) {
   return I8 ? static_cast<float>(static_cast<int32_t>(v)) : __uint_as_float(v);
 }
 
-__device__ __forceinline__ void store_one(const Params& p, int64_t i, float v) {
-  if (p.out_type == IMD_TYPE_F32) static_cast<float*>(p.out)[i] = v;
-  else if (p.out_type == IMD_TYPE_F16) static_cast<__half*>(p.out)[i] = __float2half_rn(v);
-  else static_cast<__nv_bfloat16*>(p.out)[i] = __float2bfloat16_rn(v);
-}
 template <typename T>
 __device__ __forceinline__ void store_wide(void* out, int64_t i, const float* v) {
   constexpr int V = 16 / sizeof(T);
@@ -89,12 +84,13 @@ __device__ __forceinline__ void store_wide(void* out, int64_t i, const float* v)
 // ---- many rows: CTA pairs ------------------------------------------------------------------------------
 // Signals as in the contraction's pair kernel: full[s] in the leader, armed with the bytes of both CTAs;
 // empty[s] and tfull[a] by commits that reach both CTAs; tempty[a] in the leader, eight epilogue warps.
+constexpr int kTurnBytes = 32 * 33 * 4;  // a warp's 32 x 32 block, turned for stores along the rows
 template <int BN>
 constexpr int kPairStageBytes = kBytesM + BN / 2 * kTileK;
 template <int BN>
 constexpr int kPairStages = BN == 256 ? 6 : 8;
 template <int BN>
-constexpr int kPairSmem = kPairStages<BN> * kPairStageBytes<BN> + 1024 + kCtrlBytes;
+constexpr int kPairSmem = kPairStages<BN> * kPairStageBytes<BN> + 1024 + kCtrlBytes + 4 * kTurnBytes;
 
 __device__ __forceinline__ void pair_tile(const Params& p, int w, int* tm, int* tn) {
   const int band = p.band_rows * p.tiles_n;
@@ -244,29 +240,36 @@ k_dense8_pair(const __grid_constant__ CUtensorMap map_x, const __grid_constant__
       const float xs = row < p.rows ? p.x_scale[row] : 0.0f;
       const int64_t base = static_cast<int64_t>(row) * p.out_stride;
       const uint32_t taddr = tmem_base + acc * BN + (static_cast<uint32_t>(quarter * 32) << 16);
+      float* turn = reinterpret_cast<float*>(ctrl + kCtrlBytes) + (warp - 2) * (kTurnBytes / 4);
 #pragma unroll 1
       for (int cc = 0; cc < BN; cc += 32) {
         const int col = tn * BN + cc;
         if (col >= p.n) break;  // the same for the whole warp
         uint32_t v[32];
         tmem_load_32(taddr + cc, v);
-        if (row < p.rows) {
+        if (p.out_wide && col + 32 <= p.n) {  // the same for the whole warp
+          if (row < p.rows) {
 #pragma unroll
-          for (int h = 0; h < 32; h += 16) {
-            float f[16];
+            for (int h = 0; h < 32; h += 16) {
+              float f[16];
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-              f[j] = col + h + j < p.n ? acc_value<I8>(v[h + j]) * xs * __ldg(p.w_scale + col + h + j) : 0.0f;
-            if (p.out_wide && col + h + 16 <= p.n) {
+              for (int j = 0; j < 16; ++j) f[j] = acc_value<I8>(v[h + j]) * xs * __ldg(p.w_scale + col + h + j);
               if (p.out_type == IMD_TYPE_F32) store_wide<float>(p.out, base + col + h, f);
               else if (p.out_type == IMD_TYPE_F16) store_wide<__half>(p.out, base + col + h, f);
               else store_wide<__nv_bfloat16>(p.out, base + col + h, f);
-            } else {
-#pragma unroll
-              for (int j = 0; j < 16; ++j)
-                if (col + h + j < p.n) store_one(p, base + col + h + j, f[j]);
             }
           }
+        } else {
+          // rows of the output that start anywhere: the block is turned in shared memory so that a
+          // warp stores 32 neighbours of one row (a lane's own row would touch 32 sectors a store)
+#pragma unroll
+          for (int j = 0; j < 32; ++j) turn[lane * 33 + j] = acc_value<I8>(v[j]) * xs;
+          __syncwarp();
+          const float ws = col + lane < p.n ? p.w_scale[col + lane] : 0.0f;
+          const int rows = min(32, p.rows - (row - lane));
+          for (int r = 0; r < rows; ++r)
+            if (col + lane < p.n)
+              store_out(p.out, p.out_type, static_cast<int64_t>(row - lane + r) * p.out_stride + col + lane, turn[r * 33 + lane] * ws);
         }
         __syncwarp();
       }
@@ -407,7 +410,7 @@ k_dense8_swap(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
 #pragma unroll
           for (int j = 0; j < 32; ++j)
             if (c + j < p.rows)
-              store_one(p, (c + j) * p.out_stride + n0 + row, acc_value<I8>(v[j]) * __ldg(p.x_scale + c + j) * ws);
+              store_out(p.out, p.out_type, (c + j) * p.out_stride + n0 + row, acc_value<I8>(v[j]) * __ldg(p.x_scale + c + j) * ws);
         }
         __syncwarp();
       }
@@ -437,7 +440,7 @@ k_dense8_swap(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
             const uint32_t u = load_cluster(map_to_cta(at, r));
             v = I8 ? v + u : __float_as_uint(__uint_as_float(v) + __uint_as_float(u));
           }
-          store_one(p, (c0 + c) * p.out_stride + n0 + row, acc_value<I8>(v) * p.x_scale[c0 + c] * ws);
+          store_out(p.out, p.out_type, (c0 + c) * p.out_stride + n0 + row, acc_value<I8>(v) * p.x_scale[c0 + c] * ws);
         }
       }
       __syncwarp();
@@ -527,6 +530,11 @@ bool set_attributes() {
 template <bool I8>
 bool launch(const LinearArgs& a, const DeviceInfo& dev, const Params& p, cudaStream_t stream) {
   if (a.rows <= 256) return launch_swap<I8>(a, dev, p, stream);
+  // whole waves of tiles on the CTA pairs: 128 columns where their last wave is fuller by more than the
+  // narrower tile costs
+  const int64_t tiles_m = (a.rows + 255) / 256, pairs = dev.sms / 2;
+  auto waves = [&](int64_t bn) { return (tiles_m * ((a.n + bn - 1) / bn) + pairs - 1) / pairs * bn; };
+  if (waves(128) * 115 < waves(256) * 100) return launch_pair<I8, 128>(a, dev, p, stream);
   return launch_pair<I8, 256>(a, dev, p, stream);
 }
 

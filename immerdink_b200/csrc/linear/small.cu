@@ -46,71 +46,11 @@ __device__ __forceinline__ void mma_s8(int* d, const uint32_t* a, uint32_t b0, u
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// `BYTES` bytes at p + at, zeros from `end` on. WIDE: p + at is aligned to BYTES and the whole piece
-// lies before `end` unless it starts there.
-template <int BYTES, bool WIDE>
-__device__ __forceinline__ void load_bytes(const uint8_t* p, int64_t at, int64_t end, uint32_t* v) {
-  if (WIDE && at + BYTES <= end) {
-    if (BYTES == 16) {
-      const uint4 t = *reinterpret_cast<const uint4*>(p + at);
-      v[0] = t.x, v[1 % (BYTES / 4)] = t.y, v[2 % (BYTES / 4)] = t.z, v[3 % (BYTES / 4)] = t.w;
-    } else if (BYTES == 8) {
-      const uint2 t = *reinterpret_cast<const uint2*>(p + at);
-      v[0] = t.x, v[1 % (BYTES / 4)] = t.y;
-    } else {
-      v[0] = *reinterpret_cast<const uint32_t*>(p + at);
-    }
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < BYTES / 4; ++i) {
-    uint32_t word = 0;
-#pragma unroll
-    for (int b = 0; b < 4; ++b)
-      if (at + 4 * i + b < end) word |= static_cast<uint32_t>(p[at + 4 * i + b]) << (8 * b);
-    v[i] = word;
-  }
-}
-// The same for 16-bit elements whose address is a multiple of 2 only.
-template <int WORDS, bool WIDE>
-__device__ __forceinline__ void load_halves(const uint16_t* p, int64_t at, int64_t end, uint32_t* v) {
-  if (WIDE && at + 2 * WORDS <= end) {
-#pragma unroll
-    for (int i = 0; i < WORDS; i += 4) {
-      const uint4 t = *reinterpret_cast<const uint4*>(p + at + 2 * i);
-      v[i] = t.x, v[i + 1] = t.y, v[i + 2] = t.z, v[i + 3] = t.w;
-    }
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < WORDS; ++i) {
-    uint32_t word = 0;
-    if (at + 2 * i < end) word = p[at + 2 * i];
-    if (at + 2 * i + 1 < end) word |= static_cast<uint32_t>(p[at + 2 * i + 1]) << 16;
-    v[i] = word;
-  }
-}
-
-__device__ __forceinline__ uint32_t sub_pair(uint32_t a, uint32_t b, __half) {
-  __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
-  return *reinterpret_cast<uint32_t*>(&r);
-}
-__device__ __forceinline__ uint32_t sub_pair(uint32_t a, uint32_t b, __nv_bfloat16) {
-  __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
-  return *reinterpret_cast<uint32_t*>(&r);
-}
 __device__ __forceinline__ void mma_pair(float* d, const uint32_t* a, uint32_t b0, uint32_t b1, __half) {
   mma_f16(d, a, b0, b1);
 }
 __device__ __forceinline__ void mma_pair(float* d, const uint32_t* a, uint32_t b0, uint32_t b1, __nv_bfloat16) {
   mma_bf16(d, a, b0, b1);
-}
-
-__device__ __forceinline__ void store_out(const LinearArgs& p, int64_t t, int64_t n, float v) {
-  const int64_t i = t * p.out_stride + n;
-  if (p.out_type == IMD_TYPE_F32) static_cast<float*>(p.out)[i] = v;
-  else if (p.out_type == IMD_TYPE_F16) static_cast<__half*>(p.out)[i] = __float2half_rn(v);
-  else static_cast<__nv_bfloat16*>(p.out)[i] = __float2bfloat16_rn(v);
 }
 
 // Folds the warps' partial tiles in the order of the warps and hands each output to `write`.
@@ -137,14 +77,14 @@ template <typename X, int GROUP, int NT, bool WIDE>
 __global__ void __launch_bounds__(32 * kWarps) k_small_w4(const __grid_constant__ LinearArgs p) {
   constexpr int kBytes = GROUP / 8;       // weights of one lane and row in one group
   constexpr int kWords = kBytes / 4;
-  constexpr bool kHalf = sizeof(X) == 2 && __is_same(X, __half);
-  constexpr uint32_t kMagic = kHalf ? 0x64006400u : 0x43004300u;
+  constexpr uint32_t kMagic = nibble_magic<X>();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t n0 = blockIdx.x * static_cast<int64_t>(kRowsPerTile), t0 = blockIdx.y * static_cast<int64_t>(8 * NT);
   const int64_t row[2] = {min(n0 + (lane >> 2), p.n - 1), min(n0 + (lane >> 2) + 8, p.n - 1)};
   const uint8_t* w[2] = {static_cast<const uint8_t*>(p.w) + row[0] * p.w_stride,
                          static_cast<const uint8_t*>(p.w) + row[1] * p.w_stride};
   const int64_t w_end = (p.k + 1) / 2;
+  const Span span_w = span_of(p.w, p.n, p.w_stride, w_end), span_x = span_of(p.x, p.rows, 2 * p.x_stride, 2 * p.k);
   const int64_t groups = (p.k + GROUP - 1) / GROUP;
   float acc[NT][4] = {};
   for (int64_t g = warp; g < groups; g += kWarps) {
@@ -153,7 +93,7 @@ __global__ void __launch_bounds__(32 * kWarps) k_small_w4(const __grid_constant_
     float scale[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      load_bytes<kBytes, WIDE>(w[h], k0 / 2, w_end, q[h]);
+      load_bytes<kBytes, WIDE>(w[h], k0 / 2, w_end, span_w, q[h]);
       scale[h] = load_scale(p.scale4, p.scale_type, row[h] * p.scale_stride + g);
       const uint32_t z = p.zeros == nullptr ? 8u : p.zeros[row[h] * p.zeros_stride + g] & 15u;
       zero[h] = kMagic | z | (z << 16);
@@ -163,7 +103,7 @@ __global__ void __launch_bounds__(32 * kWarps) k_small_w4(const __grid_constant_
     for (int j = 0; j < NT; ++j) {
       const int64_t t = t0 + 8 * j + (lane >> 2);
       if (t < p.rows) {
-        load_halves<4 * kWords, WIDE>(static_cast<const uint16_t*>(p.x) + t * p.x_stride, k0, p.k, &x[j][0][0]);
+        load_bytes<16 * kWords, WIDE>(static_cast<const uint8_t*>(p.x) + 2 * t * p.x_stride, 2 * k0, 2 * p.k, span_x, &x[j][0][0]);
       } else {
 #pragma unroll
         for (int i = 0; i < 4 * kWords; ++i) (&x[j][0][0])[i] = 0;
@@ -174,10 +114,7 @@ __global__ void __launch_bounds__(32 * kWarps) k_small_w4(const __grid_constant_
     for (int i = 0; i < kWords; ++i) {
       uint32_t a[2][4];  // [row][pair]: pairs (0, 4), (1, 5), (2, 6), (3, 7) of the word
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-          a[h][b] = sub_pair(((q[h][i] >> (4 * b)) & 0x000F000Fu) | kMagic, zero[h], X());
+      for (int h = 0; h < 2; ++h) nibble_pairs<X>(q[h][i], zero[h], a[h]);
       const uint32_t a01[4] = {a[0][0], a[1][0], a[0][1], a[1][1]}, a23[4] = {a[0][2], a[1][2], a[0][3], a[1][3]};
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
@@ -191,7 +128,7 @@ __global__ void __launch_bounds__(32 * kWarps) k_small_w4(const __grid_constant_
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[j][i] = fmaf(scale[i >> 1], sum[j][i], acc[j][i]);
   }
-  fold<NT, float>(acc, p, n0, t0, [&](int64_t t, int64_t n, float v) { store_out(p, t, n, v); });
+  fold<NT, float>(acc, p, n0, t0, [&](int64_t t, int64_t n, float v) { store_out(p.out, p.out_type, t * p.out_stride + n, v); });
 }
 
 // 16 e4m3 values (4 words) as f16 pairs.
@@ -214,17 +151,18 @@ __global__ void __launch_bounds__(32 * kWarps) k_small_8(const __grid_constant__
 #pragma unroll
   for (int h = 0; h < 2; ++h)
     w[h] = static_cast<const uint8_t*>(p.w) + min(n0 + (lane >> 2) + 8 * h, p.n - 1) * p.w_stride;
+  const Span span_w = span_of(p.w, p.n, p.w_stride, p.k), span_x = span_of(p.x, p.rows, p.x_stride, p.k);
   Acc acc[NT][4] = {};
   for (int64_t c = warp; c * 64 < p.k; c += kWarps) {
     const int64_t k0 = c * 64 + (lane & 3) * 16;
     uint32_t q[2][4], x[NT][4];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) load_bytes<16, WIDE>(w[h], k0, p.k, q[h]);
+    for (int h = 0; h < 2; ++h) load_bytes<16, WIDE>(w[h], k0, p.k, span_w, q[h]);
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       const int64_t t = t0 + 8 * j + (lane >> 2);
       if (t < p.rows) {
-        load_bytes<16, WIDE>(static_cast<const uint8_t*>(p.x) + t * p.x_stride, k0, p.k, x[j]);
+        load_bytes<16, WIDE>(static_cast<const uint8_t*>(p.x) + t * p.x_stride, k0, p.k, span_x, x[j]);
       } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[j][i] = 0;
@@ -252,7 +190,7 @@ __global__ void __launch_bounds__(32 * kWarps) k_small_8(const __grid_constant__
     }
   }
   fold<NT, Acc>(acc, p, n0, t0, [&](int64_t t, int64_t n, Acc v) {
-    store_out(p, t, n, static_cast<float>(v) * p.x_scale[t] * p.w_scale8[n]);
+    store_out(p.out, p.out_type, t * p.out_stride + n, static_cast<float>(v) * p.x_scale[t] * p.w_scale8[n]);
   });
 }
 

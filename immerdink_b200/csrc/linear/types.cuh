@@ -36,4 +36,88 @@ __device__ __forceinline__ float load_scale(const void* p, int32_t type, int64_t
   return to_float(static_cast<const __nv_bfloat16*>(p)[i]);
 }
 
+__device__ __forceinline__ void store_out(void* out, int32_t type, int64_t i, float v) {
+  if (type == IMD_TYPE_F32) static_cast<float*>(out)[i] = v;
+  else if (type == IMD_TYPE_F16) static_cast<__half*>(out)[i] = __float2half_rn(v);
+  else static_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(v);
+}
+
+// The addresses [lo, hi) of a matrix: what a load may touch.
+struct Span {
+  uintptr_t lo, hi;
+};
+__device__ __forceinline__ Span span_of(const void* p, int64_t rows, int64_t stride_bytes, int64_t row_bytes) {
+  const uintptr_t lo = reinterpret_cast<uintptr_t>(p);
+  return {lo, lo + static_cast<uintptr_t>((rows - 1) * stride_bytes + row_bytes)};
+}
+
+// `BYTES` bytes at row + at, zeros from `end` (the row's length in bytes) on. WIDE: row + at is aligned to
+// min(BYTES, 16). Rows of any alignment are read as the aligned words around them, shifted into place,
+// wherever those words lie inside the matrix; single bytes remain at its two ends and at a row's end.
+template <int BYTES, bool WIDE>
+__device__ __forceinline__ void load_bytes(const uint8_t* row, int64_t at, int64_t end, const Span& span, uint32_t* v) {
+  const uint8_t* p = row + at;
+  if (at + BYTES <= end) {
+    if (WIDE) {
+      if constexpr (BYTES >= 16) {
+#pragma unroll
+        for (int i = 0; i < BYTES / 4; i += 4) {
+          const uint4 t = *reinterpret_cast<const uint4*>(p + 4 * i);
+          v[i] = t.x, v[i + 1] = t.y, v[i + 2] = t.z, v[i + 3] = t.w;
+        }
+      } else if constexpr (BYTES == 8) {
+        const uint2 t = *reinterpret_cast<const uint2*>(p);
+        v[0] = t.x, v[1] = t.y;
+      } else {
+        v[0] = *reinterpret_cast<const uint32_t*>(p);
+      }
+      return;
+    }
+    const uintptr_t first = reinterpret_cast<uintptr_t>(p) & ~static_cast<uintptr_t>(3);
+    if (first >= span.lo && first + BYTES + 4 <= span.hi) {
+      const uint32_t shift = 8 * (reinterpret_cast<uintptr_t>(p) & 3);
+      const uint32_t* q = reinterpret_cast<const uint32_t*>(first);
+      uint32_t low = q[0];
+#pragma unroll
+      for (int i = 0; i < BYTES / 4; ++i) {
+        const uint32_t high = q[i + 1];
+        v[i] = __funnelshift_r(low, high, shift);
+        low = high;
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < BYTES / 4; ++i) {
+    uint32_t word = 0;
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+      if (at + 4 * i + b < end) word |= static_cast<uint32_t>(p[4 * i + b]) << (8 * b);
+    v[i] = word;
+  }
+}
+
+// 4-bit weights as exact 16-bit floats: a nibble or'ed into the mantissa of 128 (bf16) or 1024 (f16).
+template <typename X>
+__host__ __device__ constexpr uint32_t nibble_magic();
+template <>
+__host__ __device__ constexpr uint32_t nibble_magic<__half>() { return 0x64006400u; }
+template <>
+__host__ __device__ constexpr uint32_t nibble_magic<__nv_bfloat16>() { return 0x43004300u; }
+
+__device__ __forceinline__ uint32_t sub_pair(uint32_t a, uint32_t b, __half) {
+  __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t sub_pair(uint32_t a, uint32_t b, __nv_bfloat16) {
+  __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  return *reinterpret_cast<uint32_t*>(&r);
+}
+// The pairs (w_i - z, w_i+4 - z), i = 0..3, of the eight nibbles of a word; zero = magic | z | z << 16.
+template <typename X>
+__device__ __forceinline__ void nibble_pairs(uint32_t word, uint32_t zero, uint32_t* pair) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) pair[i] = sub_pair(((word >> (4 * i)) & 0x000F000Fu) | nibble_magic<X>(), zero, X());
+}
+
 }  // namespace imd
