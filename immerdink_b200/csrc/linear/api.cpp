@@ -80,7 +80,7 @@ imd_status_t imd_norm_quantize(int64_t rows, int64_t dim, int32_t x_type, const 
   a.scale = scale;
   a.x_stride = x_stride, a.residual_stride = residual_stride;
   a.residual_out_stride = residual_out_stride, a.q_stride = q_stride;
-  a.eps = static_cast<float>(eps), a.eps64 = eps;
+  a.eps = static_cast<float>(eps), a.eps_root = static_cast<float>(std::sqrt(eps));
   a.x_type = x_type, a.weight_type = weight_type, a.q_type = q_type;
   return imd::norm_quantize_launch(a, stream);
 }

@@ -12,7 +12,8 @@ struct DeviceInfo {
 // Of the current device; made on first use, nullptr where that fails (asked again at the next call).
 const DeviceInfo* device_info();
 
-// Kernel attributes on the current device; whether the tensor-core kernels take this call; the call.
+bool norm_setup();  // kernel attributes on the current device
+// The same; whether the tensor-core kernels take this call; the call.
 bool dense8_setup();
 bool dense8_takes(const LinearArgs& a);
 imd_status_t dense8_launch(const LinearArgs& a, cudaStream_t stream);

@@ -15,9 +15,9 @@ struct NormArgs {
   void *residual_out, *q;
   float* scale;
   int64_t x_stride, residual_stride, residual_out_stride, q_stride;
-  float eps;
-  double eps64;
+  float eps, eps_root;             // eps and its square root (which keeps an eps below the 32-bit range)
   int32_t x_type, weight_type, q_type;
+  unsigned int* error_word;
 };
 imd_status_t norm_quantize_launch(const NormArgs& a, cudaStream_t stream);
 

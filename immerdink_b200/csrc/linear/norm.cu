@@ -9,18 +9,29 @@
 // one CTA; rows beyond the register capacity are read three times (twice from L2).
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
+#include "dense.hpp"
+#include "cuda/sm100.cuh"
 #include "types.cuh"
 
 namespace imd {
 namespace {
 
 constexpr int kWarpRows = 4;     // rows (= warps) of a CTA in the warp-per-row form
+constexpr int kMaxSlots = 8;     // rows in flight per CTA in the ring form
+constexpr int kRingBytes = 200 * 1024;  // of one SM, shared by its CTAs
 constexpr float kTiny = 0x1p-90f, kHuge = 0x1p+120f;
 
 // Row reductions. WARP: the row belongs to one warp. Otherwise to the CTA: each warp leaves its
 // partial in shared memory, one barrier, and every warp folds the partials in the same order.
 // Consecutive reductions of a row use different slots, so one barrier each is enough.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
 template <bool WARP>
 __device__ __forceinline__ float row_sum(float v, float* slot) {
 #pragma unroll
@@ -46,30 +57,98 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* slot) {
 }
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
+// 16 bytes of a row as four words, or one element (V = 1); their values; and the reverse.
 template <typename T, int V>
-__device__ __forceinline__ void load(const void* p, int64_t i, float* f) {
-  const Pack<T, V> t = *reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(p) + i);
+struct Piece {
+  static constexpr int kWords = V == 1 ? 1 : 4;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void clear() {
 #pragma unroll
-  for (int j = 0; j < V; ++j) f[j] = to_float(t.v[j]);
-}
+    for (int i = 0; i < kWords; ++i) w[i] = 0;
+  }
+  __device__ __forceinline__ void load(const void* p, int64_t i) {
+    const T* at = static_cast<const T*>(p) + i;
+    if constexpr (V > 1) {
+      const uint4 t = *reinterpret_cast<const uint4*>(at);
+      w[0] = t.x, w[1] = t.y, w[2] = t.z, w[3] = t.w;
+    } else if constexpr (sizeof(T) == 4) {
+      w[0] = *reinterpret_cast<const uint32_t*>(at);
+    } else {
+      w[0] = *reinterpret_cast<const uint16_t*>(at);
+    }
+  }
+  __device__ __forceinline__ float value(int v) const {
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(w[v]);
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      return __uint_as_float(v % 2 != 0 ? w[v / 2] & 0xFFFF0000u : w[v / 2] << 16);
+    } else {
+      const __half2 h = *reinterpret_cast<const __half2*>(&w[v / 2]);
+      return v % 2 != 0 ? __high2float(h) : __low2float(h);
+    }
+  }
+  __device__ __forceinline__ static void store(void* p, int64_t i, const float* f) {
+    T* at = static_cast<T*>(p) + i;
+    if constexpr (V == 1) {
+      *at = from_float<T>(f[0]);
+    } else {
+      uint32_t o[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (sizeof(T) == 4) {
+          o[j] = __float_as_uint(f[j]);
+        } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+          const __nv_bfloat162 b = __floats2bfloat162_rn(f[2 * j], f[2 * j + 1]);
+          o[j] = *reinterpret_cast<const uint32_t*>(&b);
+        } else {
+          const __half2 b = __floats2half2_rn(f[2 * j], f[2 * j + 1]);
+          o[j] = *reinterpret_cast<const uint32_t*>(&b);
+        }
+      }
+      *reinterpret_cast<uint4*>(at) = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+  }
+};
+
+// V codes of the scaled values y. int8: adding 1.5 * 2^23 rounds to the nearest even integer and leaves it,
+// in two's complement, in the low bits; `keep` clears the codes of a row that has no finite scale.
 template <int V>
-__device__ __forceinline__ void store_codes(void* p, int64_t i, const float* y, bool e4m3) {
-  Pack<uint8_t, V> t;
+__device__ __forceinline__ void store_codes(void* p, int64_t i, const float* y, bool e4m3, uint32_t keep) {
+  uint8_t* at = static_cast<uint8_t*>(p) + i;
+  if constexpr (V == 1) {
+    *at = e4m3 ? static_cast<uint8_t>(__nv_cvt_float_to_fp8(y[0], __NV_SATFINITE, __NV_E4M3))
+               : static_cast<uint8_t>(__float_as_uint(y[0] + 12582912.0f) & keep);
+  } else {
+    uint32_t o[V / 4];
 #pragma unroll
-  for (int j = 0; j < V; ++j)
-    t.v[j] = e4m3 ? static_cast<uint8_t>(__nv_cvt_float_to_fp8(y[j], __NV_SATFINITE, __NV_E4M3))
-                  : static_cast<uint8_t>(y[j] != y[j] ? 0 : __float2int_rn(y[j]));
-  *reinterpret_cast<Pack<uint8_t, V>*>(static_cast<uint8_t*>(p) + i) = t;
+    for (int j = 0; j < V / 4; ++j) {
+      const float* f = y + 4 * j;
+      if (e4m3) {
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(f[0], f[1]), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(f[2], f[3]), __NV_SATFINITE, __NV_E4M3);
+        o[j] = lo | (hi << 16);
+      } else {
+        uint32_t b[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) b[c] = __float_as_uint(f[c] + 12582912.0f);
+        o[j] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410) & keep;
+      }
+    }
+    if constexpr (V == 8) *reinterpret_cast<uint2*>(at) = make_uint2(o[0], o[1]);
+    else *reinterpret_cast<uint32_t*>(at) = o[0];
+  }
 }
 
 // What turns a row's y into codes: q = round(y * pre * inv), scale as stored.
 struct RowScale {
   float pre, inv, scale;
+  uint32_t keep;  // all ones, or zero for a row without a finite scale
 };
 __device__ __forceinline__ RowScale row_scale(uint32_t top, float q_max) {
-  RowScale s{1.0f, 0.0f, 0.0f};
+  RowScale s{1.0f, 0.0f, 0.0f, ~0u};
   if (top >= 0x7F800000u) {
     s.inv = s.scale = __uint_as_float(0x7FC00000u);  // a NaN or an infinity in the row
+    s.keep = 0;
   } else if (top != 0) {
     const float a = __uint_as_float(top);
     s.scale = a / q_max;
@@ -79,181 +158,284 @@ __device__ __forceinline__ RowScale row_scale(uint32_t top, float q_max) {
   return s;
 }
 
-// 1 / sqrt(mean h^2 + eps) of a row whose squares left the 32-bit range: the row is scaled by the
-// power of two 2^-e that brings its largest entry to [1, 2), and the factor for the scaled values
-// is returned (0 rows: factor 0). `scale_down` receives 2^-e in two factors.
-struct Rescaled {
-  float f1, f2, r;
+struct Shared {
+  float sums[2][32];
+  uint32_t tops[2][32];
 };
-__device__ __forceinline__ void power_of_two(uint32_t top, Rescaled* s, int* e) {
-  *e = top == 0 ? 0 : ilogbf(__uint_as_float(top));
-  const int a = -*e / 2;
-  s->f1 = ldexpf(1.0f, a);
-  s->f2 = ldexpf(1.0f, -*e - a);
+__device__ __forceinline__ bool in_range(float ss, float eps) { return ss < kHuge && (ss >= kTiny || eps >= kTiny); }
+
+// Rows whose squares leave the 32-bit range are summed again after the exact scaling by the power of two
+// 2^-e (in two factors) that brings the largest entry to [1, 2).
+struct Down {
+  float f1, f2;
+  int e;
+};
+__device__ __forceinline__ Down scale_down(uint32_t top) {
+  const int e = ilogbf(__uint_as_float(top)), half = -e / 2;
+  return {ldexpf(1.0f, half), ldexpf(1.0f, -e - half), e};
+}
+// 1 / sqrt(mean + eps 2^-2e) for such a row; `top` is its largest magnitude (0: factor 0, so zeros stay zeros).
+__device__ __forceinline__ float root_down(float mean, float eps_root, uint32_t top, int e) {
+  if (top == 0) return 0.0f;
+  if (top >= 0x7F800000u) return __uint_as_float(0x7FC00000u);
+  const float t = ldexpf(eps_root, -e);
+  return t > 0x1p+60f ? 1.0f / t : 1.0f / sqrtf(mean + t * t);
 }
 
-template <typename T, int V, int E, bool WARP>
-__global__ void __launch_bounds__(WARP ? 32 * kWarpRows : 1024)
-k_norm_quantize(const __grid_constant__ NormArgs p) {
-  __shared__ float sums[2][32];
-  __shared__ uint32_t tops[2][32];
-  const int threads = WARP ? 32 : blockDim.x;
-  const int t = WARP ? (threadIdx.x & 31) : threadIdx.x;
-  const int64_t first = WARP ? blockIdx.x * static_cast<int64_t>(kWarpRows) + (threadIdx.x >> 5) : blockIdx.x;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * (WARP ? kWarpRows : 1);
-  const int dim = static_cast<int>(p.dim);
-  const bool e4m3 = p.q_type == IMD_TYPE_E4M3;
-  for (int64_t row = first; row < p.rows; row += step) {
-    const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
-    float h[E][V];
-    float ss = 0.0f;
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const int j = (i * threads + t) * V;
-      if (j < dim) {
-        load<T, V>(x, j, h[i]);
-      } else {
-#pragma unroll
-        for (int v = 0; v < V; ++v) h[i][v] = 0.0f;
-      }
-    }
-    if (p.residual != nullptr) {
-      const T* r = static_cast<const T*>(p.residual) + row * p.residual_stride;
-#pragma unroll
-      for (int i = 0; i < E; ++i) {
-        const int j = (i * threads + t) * V;
-        if (j < dim) {
-          float f[V];
-          load<T, V>(r, j, f);
-#pragma unroll
-          for (int v = 0; v < V; ++v) h[i][v] += f[v];
-          if (p.residual_out != nullptr) {
-            Pack<T, V> o;
-#pragma unroll
-            for (int v = 0; v < V; ++v) o.v[v] = from_float<T>(h[i][v]);
-            *reinterpret_cast<Pack<T, V>*>(static_cast<T*>(p.residual_out) + row * p.residual_out_stride + j) = o;
-          }
-        }
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < E; ++i)
-#pragma unroll
-      for (int v = 0; v < V; ++v) ss = fmaf(h[i][v], h[i][v], ss);
-    ss = row_sum<WARP>(ss, sums[0]);
-    float r = 1.0f / sqrtf(ss / static_cast<float>(dim) + p.eps);
-    if (!(ss < kHuge) || (ss < kTiny && p.eps < kTiny)) {  // uniform over the row
-      uint32_t top = 0;
-#pragma unroll
-      for (int i = 0; i < E; ++i)
-#pragma unroll
-        for (int v = 0; v < V; ++v) top = max(top, magnitude(h[i][v]));
-      top = row_max<WARP>(top, tops[0]);
-      r = 0.0f;
-      if (top >= 0x7F800000u) {
-        r = __uint_as_float(0x7FC00000u);
-      } else if (top != 0) {
-        Rescaled s;
-        int e;
-        power_of_two(top, &s, &e);
-        ss = 0.0f;
-#pragma unroll
-        for (int i = 0; i < E; ++i)
-#pragma unroll
-          for (int v = 0; v < V; ++v) {
-            h[i][v] = h[i][v] * s.f1 * s.f2;
-            ss = fmaf(h[i][v], h[i][v], ss);
-          }
-        ss = row_sum<WARP>(ss, sums[1]);
-        r = static_cast<float>(1.0 / sqrt(static_cast<double>(ss) / dim + p.eps64 * exp2(-2.0 * e)));
-      }
-    }
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const int j = (i * threads + t) * V;
-      if (j < dim) {
-        float w[V];
-        if (p.weight_type == p.x_type) {
-          load<T, V>(p.weight, j, w);
-        } else {
-#pragma unroll
-          for (int v = 0; v < V; ++v) w[v] = static_cast<const float*>(p.weight)[j + v];
-        }
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          h[i][v] = h[i][v] * r * w[v];
-          top = max(top, magnitude(h[i][v]));
-        }
-      }
-    }
-    const RowScale s = row_scale(row_max<WARP>(top, tops[1]), e4m3 ? 448.0f : 127.0f);
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const int j = (i * threads + t) * V;
-      if (j < dim) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) h[i][v] = h[i][v] * s.pre * s.inv;
-        store_codes<V>(static_cast<uint8_t*>(p.q) + row * p.q_stride, j, h[i], e4m3);
-      }
-    }
-    if (t == 0) p.scale[row] = s.scale;
-  }
-}
-
-// Rows of any length: the row is read once per reduction and once for the codes; residual_out is
-// written in the last pass, by the thread that reads the same elements, so it may be x or residual.
+// Rows of any length, by repeated passes over memory, element by element. residual_out is written in the last
+// pass, by the thread that reads the same element, so it may be x or residual.
 template <typename T>
 __global__ void __launch_bounds__(1024) k_norm_quantize_long(const __grid_constant__ NormArgs p) {
-  __shared__ float sums[2][32];
-  __shared__ uint32_t tops[2][32];
+  __shared__ Shared s;
   const bool e4m3 = p.q_type == IMD_TYPE_E4M3;
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
     const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
     const T* res = p.residual == nullptr ? nullptr : static_cast<const T*>(p.residual) + row * p.residual_stride;
     auto sum = [&](int64_t j) { return to_float(x[j]) + (res != nullptr ? to_float(res[j]) : 0.0f); };
     auto weight = [&](int64_t j) {
-      return p.weight_type == p.x_type ? to_float(static_cast<const T*>(p.weight)[j])
-                                       : static_cast<const float*>(p.weight)[j];
+      return p.weight_type == p.x_type ? to_float(static_cast<const T*>(p.weight)[j]) : static_cast<const float*>(p.weight)[j];
     };
+    Down d{1.0f, 1.0f, 0};
     float ss = 0.0f;
     for (int64_t j = threadIdx.x; j < p.dim; j += blockDim.x) {
       const float h = sum(j);
       ss = fmaf(h, h, ss);
     }
-    ss = row_sum<false>(ss, sums[0]);
-    Rescaled f{1.0f, 1.0f, 1.0f / sqrtf(ss / static_cast<float>(p.dim) + p.eps)};
-    if (!(ss < kHuge) || (ss < kTiny && p.eps < kTiny)) {
+    ss = row_sum<false>(ss, s.sums[0]);
+    float r = 1.0f / sqrtf(ss / static_cast<float>(p.dim) + p.eps);
+    if (!in_range(ss, p.eps)) {  // uniform over the row
       uint32_t top = 0;
       for (int64_t j = threadIdx.x; j < p.dim; j += blockDim.x) top = max(top, magnitude(sum(j)));
-      top = row_max<false>(top, tops[0]);
-      f.r = 0.0f;
-      if (top >= 0x7F800000u) {
-        f.r = __uint_as_float(0x7FC00000u);
-      } else if (top != 0) {
-        int e;
-        power_of_two(top, &f, &e);
-        ss = 0.0f;
-        for (int64_t j = threadIdx.x; j < p.dim; j += blockDim.x) {
-          const float h = sum(j) * f.f1 * f.f2;
-          ss = fmaf(h, h, ss);
-        }
-        ss = row_sum<false>(ss, sums[1]);
-        f.r = static_cast<float>(1.0 / sqrt(static_cast<double>(ss) / p.dim + p.eps64 * exp2(-2.0 * e)));
+      top = row_max<false>(top, s.tops[0]);
+      if (top != 0 && top < 0x7F800000u) d = scale_down(top);
+      ss = 0.0f;
+      for (int64_t j = threadIdx.x; j < p.dim; j += blockDim.x) {
+        const float h = sum(j) * d.f1 * d.f2;
+        ss = fmaf(h, h, ss);
       }
+      ss = row_sum<false>(ss, s.sums[1]);
+      r = root_down(ss / static_cast<float>(p.dim), p.eps_root, top, d.e);
     }
     uint32_t top = 0;
-    for (int64_t j = threadIdx.x; j < p.dim; j += blockDim.x)
-      top = max(top, magnitude(sum(j) * f.f1 * f.f2 * f.r * weight(j)));
-    const RowScale s = row_scale(row_max<false>(top, tops[1]), e4m3 ? 448.0f : 127.0f);
+    for (int64_t j = threadIdx.x; j < p.dim; j += blockDim.x) top = max(top, magnitude(sum(j) * d.f1 * d.f2 * r * weight(j)));
+    const RowScale q = row_scale(row_max<false>(top, s.tops[1]), e4m3 ? 448.0f : 127.0f);
     for (int64_t j = threadIdx.x; j < p.dim; j += blockDim.x) {
       const float h = sum(j);
-      if (p.residual_out != nullptr)
-        static_cast<T*>(p.residual_out)[row * p.residual_out_stride + j] = from_float<T>(h);
-      const float y = h * f.f1 * f.f2 * f.r * weight(j) * s.pre * s.inv;
-      store_codes<1>(static_cast<uint8_t*>(p.q) + row * p.q_stride, j, &y, e4m3);
+      if (p.residual_out != nullptr) static_cast<T*>(p.residual_out)[row * p.residual_out_stride + j] = from_float<T>(h);
+      const float y = h * d.f1 * d.f2 * r * weight(j) * q.pre * q.inv;
+      store_codes<1>(static_cast<uint8_t*>(p.q) + row * p.q_stride, j, &y, e4m3, q.keep);
     }
-    if (threadIdx.x == 0) p.scale[row] = s.scale;
+    if (threadIdx.x == 0) p.scale[row] = q.scale;
+  }
+}
+
+// From the 32-bit sums h of a row to its outputs; E vectors of V elements per thread. `loaded` is called once,
+// after the first reduction: every thread of the row has then taken its h from wherever the row was.
+template <typename T, int V, int E, bool WARP, typename Loaded>
+__device__ __forceinline__ void finish_row(const NormArgs& p, int64_t row, int threads, int t, float (*h)[V], Shared& s,
+                                           Loaded loaded) {
+  const int dim = static_cast<int>(p.dim);
+  const bool e4m3 = p.q_type == IMD_TYPE_E4M3, same = p.weight_type == p.x_type;
+  Piece<T, V> w[E];
+      if (p.residual_out != nullptr) {
+        T* out = static_cast<T*>(p.residual_out) + row * p.residual_out_stride;
+  #pragma unroll
+        for (int i = 0; i < E; ++i) {
+          const int j = (i * threads + t) * V;
+          if (j < dim) Piece<T, V>::store(out, j, h[i]);
+        }
+      }
+      if (same) {
+  #pragma unroll
+        for (int i = 0; i < E; ++i) {
+          const int j = (i * threads + t) * V;
+          w[i].clear();
+          if (j < dim) w[i].load(p.weight, j);
+        }
+      }
+      float r;
+      for (uint32_t top = ~0u, e = 0;;) {  // a second time only for rows that leave the range
+        float ss = 0.0f;
+  #pragma unroll
+        for (int i = 0; i < E; ++i)
+  #pragma unroll
+          for (int v = 0; v < V; ++v) ss = fmaf(h[i][v], h[i][v], ss);
+        ss = row_sum<WARP>(ss, s.sums[top == ~0u ? 0 : 1]);
+    if (top == ~0u) loaded();
+        const float mean = ss / static_cast<float>(dim);
+        if (top != ~0u) {
+          r = root_down(mean, p.eps_root, top, static_cast<int>(e));
+          break;
+        }
+        if (in_range(ss, p.eps)) {
+          r = 1.0f / sqrtf(mean + p.eps);
+          break;
+        }
+        top = 0;
+  #pragma unroll
+        for (int i = 0; i < E; ++i)
+  #pragma unroll
+          for (int v = 0; v < V; ++v) top = max(top, magnitude(h[i][v]));
+        top = row_max<WARP>(top, s.tops[0]);
+        if (top != 0 && top < 0x7F800000u) {
+          const Down d = scale_down(top);
+          e = static_cast<uint32_t>(d.e);
+  #pragma unroll
+          for (int i = 0; i < E; ++i)
+  #pragma unroll
+            for (int v = 0; v < V; ++v) h[i][v] = h[i][v] * d.f1 * d.f2;
+        }
+      }
+      uint32_t top = 0;
+      if (same) {
+  #pragma unroll
+        for (int i = 0; i < E; ++i)
+  #pragma unroll
+          for (int v = 0; v < V; ++v) h[i][v] = h[i][v] * r * w[i].value(v);
+      } else {
+  #pragma unroll
+        for (int i = 0; i < E; ++i) {
+          const int j = (i * threads + t) * V;
+  #pragma unroll
+          for (int v = 0; v < V; ++v)
+            if (j < dim) h[i][v] = h[i][v] * r * static_cast<const float*>(p.weight)[j + v];
+        }
+      }
+  #pragma unroll
+      for (int i = 0; i < E; ++i)
+  #pragma unroll
+        for (int v = 0; v < V; ++v) top = max(top, magnitude(h[i][v]));
+      const RowScale c = row_scale(row_max<WARP>(top, s.tops[1]), e4m3 ? 448.0f : 127.0f);
+  #pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const int j = (i * threads + t) * V;
+        if (j < dim) {
+  #pragma unroll
+          for (int v = 0; v < V; ++v) h[i][v] = h[i][v] * c.pre * c.inv;
+          store_codes<V>(static_cast<uint8_t*>(p.q) + row * p.q_stride, j, h[i], e4m3, c.keep);
+        }
+      }
+      if (t == 0) p.scale[row] = c.scale;
+}
+
+// Rows in registers, one per warp or per CTA.
+template <typename T, int V, int E, bool WARP>
+__global__ void __launch_bounds__(WARP ? 32 * kWarpRows : E <= 2 ? 1024 : 512)
+k_norm_quantize(const __grid_constant__ NormArgs p) {
+  __shared__ Shared s;
+  const int threads = WARP ? 32 : blockDim.x;
+  const int t = WARP ? (threadIdx.x & 31) : threadIdx.x;
+  const int64_t first = WARP ? blockIdx.x * static_cast<int64_t>(kWarpRows) + (threadIdx.x >> 5) : blockIdx.x;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * (WARP ? kWarpRows : 1);
+  const int dim = static_cast<int>(p.dim);
+  for (int64_t row = first; row < p.rows; row += step) {
+    // every load of the row is issued before its first store: residual_out may be x or residual
+    const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
+    Piece<T, V> in[E], res[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const int j = (i * threads + t) * V;
+      in[i].clear();
+      if (j < dim) in[i].load(x, j);
+    }
+    if (p.residual != nullptr) {
+      const T* r = static_cast<const T*>(p.residual) + row * p.residual_stride;
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const int j = (i * threads + t) * V;
+        res[i].clear();
+        if (j < dim) res[i].load(r, j);
+      }
+    }
+    float h[E][V];
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+#pragma unroll
+      for (int v = 0; v < V; ++v) h[i][v] = in[i].value(v);
+    if (p.residual != nullptr) {
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+#pragma unroll
+        for (int v = 0; v < V; ++v) h[i][v] += res[i].value(v);
+    }
+    finish_row<T, V, E, WARP>(p, row, threads, t, h, s, [] {});
+  }
+}
+
+// Many rows: a persistent CTA whose rows arrive by bulk copies in a ring of shared memory, so that the bytes
+// in flight do not depend on registers and the next rows arrive while this one is reduced and stored. A slot
+// is refilled right after the row's first reduction, whose barrier says that every thread has read it.
+template <typename T, int V, int E>
+__global__ void __launch_bounds__(512, 2) k_norm_quantize_ring(const __grid_constant__ NormArgs p, int slots) {
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ Shared s;
+  __shared__ uint64_t bars[kMaxSlots];
+  __shared__ int gave_up;
+  const int threads = blockDim.x, t = threadIdx.x, dim = static_cast<int>(p.dim);
+  const uint32_t row_bytes = static_cast<uint32_t>(dim) * sizeof(T);
+  const uint32_t slot_bytes = row_bytes * (p.residual != nullptr ? 2 : 1);
+  volatile int* abort = &gave_up;
+  auto fetch = [&](int64_t row, int slot) {
+    const uint32_t bar = smem_u32(&bars[slot]), dst = smem_u32(ring) + slot * slot_bytes;
+    mbar_expect_tx(bar, slot_bytes);
+    bulk_load(dst, static_cast<const T*>(p.x) + row * p.x_stride, row_bytes, bar);
+    if (p.residual != nullptr)
+      bulk_load(dst + row_bytes, static_cast<const T*>(p.residual) + row * p.residual_stride, row_bytes, bar);
+  };
+  if (t == 0) {
+    gave_up = 0;
+    for (int i = 0; i < slots; ++i) mbar_init(smem_u32(&bars[i]), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    for (int i = 0; i < slots; ++i) {
+      const int64_t row = blockIdx.x + static_cast<int64_t>(i) * gridDim.x;
+      if (row < p.rows) fetch(row, i);
+    }
+  }
+  __syncthreads();
+  int slot = 0;
+  uint32_t phase = 0;
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    mbar_wait(smem_u32(&bars[slot]), phase, abort);
+    const T* x = reinterpret_cast<const T*>(ring + slot * slot_bytes);
+    float h[E][V];
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const int j = (i * threads + t) * V;
+      Piece<T, V> in;
+      in.clear();
+      if (j < dim) in.load(x, j);
+#pragma unroll
+      for (int v = 0; v < V; ++v) h[i][v] = in.value(v);
+    }
+    if (p.residual != nullptr) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const int j = (i * threads + t) * V;
+        Piece<T, V> res;
+        res.clear();
+        if (j < dim) res.load(x + dim, j);
+#pragma unroll
+        for (int v = 0; v < V; ++v) h[i][v] += res.value(v);
+      }
+    }
+    finish_row<T, V, E, false>(p, row, threads, t, h, s, [&] {
+      const int64_t next = row + static_cast<int64_t>(slots) * gridDim.x;
+      if (t == 0 && next < p.rows) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        fetch(next, slot);
+      }
+    });
+    if (++slot == slots) {
+      slot = 0;
+      phase ^= 1u;
+    }
+  }
+  if (t == 0 && *abort) {
+    // copies still in flight get a bounded time to land before their memory is given back
+    for (int i = 0; i < slots; ++i)
+      for (uint32_t it = 0; it < (1u << 20); ++it)
+        if (mbar_try_wait(smem_u32(&bars[i]), 0) || mbar_try_wait(smem_u32(&bars[i]), 1)) break;
+    atomicOr(p.error_word, 1u);
   }
 }
 
@@ -271,8 +453,11 @@ bool launch_registers(const NormArgs& a, cudaStream_t stream) {
     return true;
   }
   constexpr int kMost = V == 1 ? 16 : 4;
-  const int64_t per_thread = vecs <= 1024 ? 1 : vecs <= 2048 ? 2 : kMost;
-  if (vecs > 1024 * kMost) return false;
+  if (vecs > 512 * kMost) return false;
+  // with rows to fill the GPU, few threads with many loads in flight each; else as many threads as help
+  const int64_t least = a.rows >= 512 ? 2 : 1;
+  int64_t per_thread = vecs <= 1024 ? 1 : vecs <= 2048 ? 2 : kMost;
+  if (per_thread < least) per_thread = least;
   const int threads = static_cast<int>(((vecs + per_thread - 1) / per_thread + 31) / 32 * 32);
   const unsigned int grid = grid_of(a.rows);
   if (per_thread == 1) k_norm_quantize<T, V, 1, false><<<grid, threads, 0, stream>>>(a);
@@ -281,8 +466,29 @@ bool launch_registers(const NormArgs& a, cudaStream_t stream) {
   return true;
 }
 
+// The ring form: rows enough for every CTA slot of the GPU to take several.
+template <typename T, int V, int E>
+bool launch_ring(const NormArgs& a, const DeviceInfo& dev, int least_per_sm, cudaStream_t stream) {
+  const int64_t vecs = a.dim / V;
+  const int threads = static_cast<int>(((vecs + E - 1) / E + 31) / 32 * 32);
+  if (threads > 512) return false;
+  const int64_t slot_bytes = a.dim * static_cast<int64_t>(sizeof(T)) * (a.residual != nullptr ? 2 : 1);
+  int64_t per_sm = 1024 / threads;
+  if (per_sm > kRingBytes / (2 * slot_bytes)) per_sm = kRingBytes / (2 * slot_bytes);
+  if (per_sm < least_per_sm) return false;
+  int64_t slots = kRingBytes / per_sm / slot_bytes;
+  if (slots > kMaxSlots) slots = kMaxSlots;
+  const int64_t ctas = static_cast<int64_t>(dev.sms) * per_sm;
+  if (a.rows < 3 * ctas) return false;
+  k_norm_quantize_ring<T, V, E><<<static_cast<unsigned int>(ctas), threads, slots * slot_bytes, stream>>>(a, static_cast<int>(slots));
+  return true;
+}
+
 template <typename T>
-imd_status_t launch(const NormArgs& a, cudaStream_t stream) {
+imd_status_t launch(NormArgs a, cudaStream_t stream) {
+  const DeviceInfo* dev = device_info();
+  if (dev == nullptr) return IMD_STATUS_CUDA_ERROR;
+  a.error_word = dev->error_word;
   constexpr int V = 16 / sizeof(T);
   auto wide = [](const void* p, int64_t stride, int size, int64_t rows) {
     const uintptr_t unit = static_cast<uintptr_t>(V) * size;
@@ -293,12 +499,25 @@ imd_status_t launch(const NormArgs& a, cudaStream_t stream) {
                    wide(a.residual, a.residual_stride, sizeof(T), a.rows) &&
                    wide(a.residual_out, a.residual_out_stride, sizeof(T), a.rows) &&
                    wide(a.q, a.q_stride, 1, a.rows) && reinterpret_cast<uintptr_t>(a.weight) % (V * sw) == 0;
+  if (vec && a.dim / V > 64 &&
+      (launch_ring<T, V, 4>(a, *dev, 4, stream) || launch_ring<T, V, 2>(a, *dev, 2, stream) || launch_ring<T, V, 4>(a, *dev, 1, stream)))
+    return cudaGetLastError() == cudaSuccess ? IMD_STATUS_SUCCESS : IMD_STATUS_CUDA_ERROR;
   if (!(vec ? launch_registers<T, V>(a, stream) : launch_registers<T, 1>(a, stream)))
     k_norm_quantize_long<T><<<grid_of(a.rows), 1024, 0, stream>>>(a);
   return cudaGetLastError() == cudaSuccess ? IMD_STATUS_SUCCESS : IMD_STATUS_CUDA_ERROR;
 }
 
 }  // namespace
+
+bool norm_setup() {
+  auto smem = [](auto* f) {
+    return cudaFuncSetAttribute(reinterpret_cast<const void*>(f), cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes) ==
+           cudaSuccess;
+  };
+  return smem(k_norm_quantize_ring<float, 4, 2>) && smem(k_norm_quantize_ring<float, 4, 4>) &&
+         smem(k_norm_quantize_ring<__half, 8, 2>) && smem(k_norm_quantize_ring<__half, 8, 4>) &&
+         smem(k_norm_quantize_ring<__nv_bfloat16, 8, 2>) && smem(k_norm_quantize_ring<__nv_bfloat16, 8, 4>);
+}
 
 imd_status_t norm_quantize_launch(const NormArgs& a, cudaStream_t stream) {
   if (a.x_type == IMD_TYPE_F32) return launch<float>(a, stream);

@@ -146,6 +146,27 @@ def test_norm_range(dim, to):
     assert torch.isnan(s[1:]).all()
 
 
+@pytest.mark.parametrize("t, dim", [(BF16, 520), (F16, 1024), (F32, 1028), (BF16, 4096), (F32, 4100), (BF16, 8200), (F16, 16384), (F32, 8192), (BF16, 20480)])
+def test_norm_rows_in_a_ring(t, dim):
+    """Many rows (those that leave the range among them), with and without a residual, in place, broadcast."""
+    rows = 5003
+    x, w = rnd(11, rows, dim, dtype=t), rnd(12, dim, dtype=t)
+    r = rnd(13, 1, dim, dtype=t).expand(rows, dim)
+    if t == F32:
+        x[17] *= 1e30
+        x[4000] *= 1e-35
+    x[99], x[1234, dim - 1] = 0, math.nan
+    q, s = torch.empty(rows, dim, dtype=E4M3, device="cuda"), torch.empty(rows, device="cuda")
+    good = [i for i in range(rows) if i not in (99, 1234)]
+    imd.norm_quantize(x, w, q, s, eps=0.0)
+    assert float(s[99]) == 0 and bool(torch.isnan(s[1234]))
+    norm_check(x[good], None, w, q[good], s[good], None, 0.0, t)
+    h = x.clone()
+    imd.norm_quantize(h, w, q, s, eps=0.0, residual=r, residual_out=h)
+    good = [i for i in range(rows) if i != 1234]
+    norm_check(x[good], r[good], w, q[good], s[good], h[good], 0.0, t)
+
+
 def test_norm_many_rows():
     rows, dim = 70001, 40
     x, w = rnd(9, rows, dim, dtype=BF16), rnd(10, dim, dtype=BF16)
