@@ -30,7 +30,7 @@ HOST_SOURCES = [os.path.join(CSRC, "host", f)
 CUDA_SOURCES = [os.path.join(CSRC, "cuda", f)
                 for f in ("api.cpp", "pipeline.cu", "gemm_tcgen05.cu")]
 
-LINEAR_SOURCES = [os.path.join(CSRC, "linear", f) for f in ("api.cpp", "device.cu", "norm.cu", "small.cu", "dense8.cu", "dense4.cu")]
+LINEAR_SOURCES = [os.path.join(CSRC, "linear", f) for f in ("api.cpp", "device.cu", "norm.cu", "small.cu", "stream.cu", "dense8.cu", "dense4.cu")]
 
 
 def _cxx():

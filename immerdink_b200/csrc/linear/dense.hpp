@@ -13,10 +13,13 @@ struct DeviceInfo {
 const DeviceInfo* device_info();
 
 bool norm_setup();  // kernel attributes on the current device
-// The same; whether the tensor-core kernels take this call; the call.
+// The same; whether these kernels take this call; the call.
 bool dense8_setup();
 bool dense8_takes(const LinearArgs& a);
 imd_status_t dense8_launch(const LinearArgs& a, cudaStream_t stream);
+bool stream_setup();
+bool stream_takes(const LinearArgs& a);
+imd_status_t stream_launch(const LinearArgs& a, cudaStream_t stream);
 bool dense4_setup();
 bool dense4_takes(const LinearArgs& a);
 imd_status_t dense4_launch(const LinearArgs& a, cudaStream_t stream);

@@ -10,7 +10,8 @@
 // lane of tensor memory, so its scale is one register.
 //
 // Warpgroups (512 threads, 128 registers each at launch, shared out again by setmaxnreg):
-//   0     warp 0 brings x by TMA (64 k = 128 bytes of a row, 128-byte swizzle), warp 1 issues the MMAs
+//   0     warp 0 brings x by TMA (64 k = 128 bytes of a row, 128-byte swizzle), warp 1 issues the MMAs, warp 2
+//         brings the packed weights by TMA, 256 k (128 bytes of a row) at a time into two slots of their own
 //   1     thread r turns row r of the weights' next 64 k into 16-bit floats in the swizzled layout
 //   2, 3  halves of the rows of x: out += scale * accumulator, then the stores
 // Bound by shared memory traffic for many rows (the operand tiles are written and read at about the port's rate),
@@ -29,21 +30,23 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kRegsLaunch = 128;                                   // 65536 / kThreads
-constexpr int kRegsIssue = 40, kRegsUnpack = 104, kRegsSum = 176;  // per thread of warpgroup 0, 1, 2 and 3
+constexpr int kRegsIssue = 40, kRegsUnpack = 88, kRegsSum = 192;  // per thread of warpgroup 0, 1, 2 and 3
 static_assert(kRegsIssue + kRegsUnpack + 2 * kRegsSum <= 4 * kRegsLaunch, "register shares above the launch's total");
 constexpr int kTileM = 128, kTileN = 256;
 constexpr int kBlockK = 64;                                        // k of one pipeline stage: 128 bytes a row
 constexpr int kBytesM = kTileM * 128;
 constexpr int kMaxStages = 8;
 constexpr int kCtrlBytes = 256;
-constexpr int kSmem = 200 * 1024;
+constexpr int kSmem = 227 * 1024;
+constexpr int kChunkBlocks = 4;                                    // 64-k blocks of one packed chunk
+constexpr int kChunkBytes = kTileM * 128;
 
 struct Params {
   LinearArgs a;
   int32_t units;                  // K in steps of max(group, 64)
   int32_t tiles_t, cols, stages;  // row tiles of x; rows of x per tile, padded to 16
   int32_t acc_cols;               // tensor-memory columns of one accumulator, a power of two
-  int32_t wide;                   // rows of w are 16-byte aligned
+  int32_t wide;                   // rows of w are 16-byte aligned: they come by TMA
   unsigned int* error_word;
 };
 
@@ -61,16 +64,27 @@ __device__ __forceinline__ uint32_t load_cluster(uint32_t addr) {
   return v;
 }
 
+__device__ __forceinline__ uint64_t pair(uint32_t lo, uint32_t hi) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
+  return v;
+}
+__device__ __forceinline__ float half_of(uint64_t v, int high) {
+  return __uint_as_float(static_cast<uint32_t>(high != 0 ? v >> 32 : v));
+}
+
 template <typename X, int GROUP>
 __global__ void __launch_bounds__(kThreads, 1)
-k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ Params p) {
+k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+         const __grid_constant__ Params p) {
   constexpr int kUnit = GROUP > kBlockK ? GROUP : kBlockK;       // k of one step of the split
   constexpr int kBlocks = kUnit / kBlockK, kGroups = kUnit / GROUP;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t tiles = (raw + 1023u) & ~1023u;
   const int stage_bytes = kBytesM + p.cols * 128;
-  uint8_t* ctrl = smem_raw + (tiles - raw) + p.stages * stage_bytes;
+  const uint32_t packed = tiles + p.stages * stage_bytes;         // two chunks of packed weights
+  uint8_t* ctrl = smem_raw + (packed - raw) + 2 * kChunkBytes;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ctrl + 216);
   volatile int* abort = reinterpret_cast<volatile int*>(ctrl + 224);
   const uint32_t bar0 = smem_u32(ctrl);
@@ -78,7 +92,9 @@ k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ Para
   auto empty = [&](int s) { return bar0 + 8u * (kMaxStages + s); };
   auto tfull = [&](int a) { return bar0 + 8u * (2 * kMaxStages + a); };
   auto tempty = [&](int a) { return bar0 + 8u * (2 * kMaxStages + 2 + a); };
-  const uint32_t drain = bar0 + 8u * (2 * kMaxStages + 4);
+  auto wfull = [&](int c) { return bar0 + 8u * (2 * kMaxStages + 4 + c); };
+  auto wempty = [&](int c) { return bar0 + 8u * (2 * kMaxStages + 6 + c); };
+  const uint32_t drain = bar0 + 8u * (2 * kMaxStages + 8);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wg = warp >> 2;
   const int parts = gridDim.y, part = blockIdx.y;
@@ -94,6 +110,8 @@ k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ Para
     for (int a = 0; a < 2; ++a) {
       mbar_init(tfull(a), 1);
       mbar_init(tempty(a), 8);
+      mbar_init(wfull(a), 1);
+      mbar_init(wempty(a), 4);
     }
     mbar_init(drain, 1);
     *abort = 0;
@@ -142,12 +160,14 @@ k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ Para
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool okay = true;
+#pragma unroll 1
       for (int kb = u0 * kBlocks; kb < u1 * kBlocks && okay; ++kb) {
         if (!mbar_wait(full(stage), phase, abort)) break;
         tc_fence_after();
         const uint32_t a = tiles + stage * stage_bytes, b = a + kBytesM;
+        uint64_t da = smem_desc(a), db = smem_desc(b);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {  // 16 k an instruction
+        for (int i = 0; i < 4; ++i, da += 2, db += 2) {  // 16 k = 32 bytes an instruction
           const int at = (kb % kBlocks) * kBlockK + 16 * i;  // place in the unit
           if (at % GROUP == 0) {
             if (!mbar_wait(tempty(acc), acc_phase ^ 1u, abort)) {
@@ -156,7 +176,7 @@ k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ Para
             }
             tc_fence_after();
           }
-          mma16<X>(tmem_base + acc * p.acc_cols, smem_desc(a + 32 * i), smem_desc(b + 32 * i), idesc, at % GROUP != 0);
+          mma16<X>(tmem_base + acc * p.acc_cols, da, db, idesc, at % GROUP != 0);
           if ((at + 16) % GROUP == 0) {
             tc_commit(tfull(acc));
             acc ^= 1;
@@ -172,6 +192,21 @@ k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ Para
       tc_commit(drain);
       for (uint32_t it = 0; it < kSpinLimit; ++it)
         if (mbar_try_wait(drain, 0)) break;
+    } else if (warp == 2 && lane == 0 && p.wide) {
+      const uint64_t policy = l2_policy(0);
+      const int chunks = ((u1 - u0) * kBlocks + kChunkBlocks - 1) / kChunkBlocks;
+      int c = 0;
+      for (; c < chunks; ++c) {
+        const int slot = c & 1;
+        if (!mbar_wait(wempty(slot), ((c >> 1) & 1) ^ 1u, abort)) break;
+        mbar_expect_tx(wfull(slot), kChunkBytes);
+        tma_load_3d(packed + slot * kChunkBytes, &map_w, wfull(slot), (u0 * kBlocks + c * kChunkBlocks) * (kBlockK / 2),
+                    static_cast<int>(n0), 0, policy);
+      }
+      if (c < chunks)  // as above: the copies of the last two chunks
+        for (int s = 0; s < 2 && s < c; ++s)
+          for (uint32_t it = 0; it < (1u << 20); ++it)
+            if (mbar_try_wait(wfull(s), 0) || mbar_try_wait(wfull(s), 1)) break;
     }
     __syncwarp();
   } else if (wg == 1) {
@@ -183,42 +218,73 @@ k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ Para
     const int64_t end = (p.a.k + 1) / 2;
     const int groups = static_cast<int>((p.a.k + GROUP - 1) / GROUP);
     const Span span = span_of(p.a.w, p.a.n, p.a.w_stride, end);
-    auto fetch = [&](int kb, uint32_t* q) {
-      const int64_t at = static_cast<int64_t>(kb) * (kBlockK / 2);
-      if (p.wide) load_bytes<32, true>(w, at, end, span, q);
-      else load_bytes<32, false>(w, at, end, span, q);
+    // a chunk's zero points (four bits each) and, for rows of any alignment, a block's weights are loaded one
+    // step ahead
+    constexpr int kZeros = kChunkBlocks * kBlockK / GROUP;
+    uint32_t zero_next[kZeros];
+    auto fetch_zeros = [&](int kb) {
+      const int g0 = kb * kBlockK / GROUP;
+#pragma unroll
+      for (int i = 0; i < kZeros; ++i) zero_next[i] = zeros == nullptr ? 8u : g0 + i < groups ? zeros[g0 + i] : 0u;
     };
-    uint32_t next[8];
-    const int kb1 = u1 * kBlocks;
+    const int kb0 = u0 * kBlocks, kb1 = u1 * kBlocks;
+    const uint32_t own = packed + r * 128;  // this row in the packed chunks
+    // rows of any alignment: each thread brings its own row's chunk to the place where TMA would put it
+    auto fetch_row = [&](int kb, int slot) {
+#pragma unroll 1
+      for (int i = 0; i < 8; ++i) {
+        uint32_t q[4];
+        load_bytes<16>(w, static_cast<int64_t>(kb) * (kBlockK / 2) + 16 * i, end, span, q);
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(own + slot * kChunkBytes + ((i ^ (r & 7)) << 4)),
+                     "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3])
+                     : "memory");
+      }
+    };
     int stage = 0;
-    uint32_t phase = 0;
-    if (u0 < u1) fetch(u0 * kBlocks, next);
-    for (int kb = u0 * kBlocks; kb < kb1; ++kb) {
-      uint32_t q[8];
+    uint32_t phase = 0, zero_bits = 0;
+    fetch_zeros(kb0);
+    if (!p.wide) fetch_row(kb0, 0);
+    // Rolled, as are the other roles' loops: one warp of each scheduler runs this code, so what does not fit the
+    // smallest instruction cache is fetched again at every turn (unrolled over a block: 1400 cycles a block).
+#pragma unroll 1
+    for (int kb = kb0; kb < kb1; ++kb) {
+      const int b = (kb - kb0) % kChunkBlocks, c = (kb - kb0) / kChunkBlocks;
+      if (b == 0) {
+        zero_bits = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) q[i] = next[i];
-      if (kb + 1 < kb1) fetch(kb + 1, next);
-      uint32_t zero[2];  // of the first and the second 32 k
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int g = (kb * kBlockK + 32 * h) / GROUP;
-        const uint32_t z = zeros == nullptr ? 8u : g < groups ? zeros[g] & 15u : 0u;
-        zero[h] = nibble_magic<X>() | z | (z << 16);
+        for (int i = 0; i < kZeros; ++i) zero_bits |= (zero_next[i] & 15u) << (4 * i);
+        if (kb + kChunkBlocks < kb1) {
+          fetch_zeros(kb + kChunkBlocks);
+          if (!p.wide) fetch_row(kb + kChunkBlocks, (c + 1) & 1);
+        }
+        if (p.wide && !mbar_wait(wfull(c & 1), (c >> 1) & 1, abort)) break;
       }
       if (!mbar_wait(empty(stage), phase ^ 1u, abort)) break;
-      const uint32_t dst = tiles + stage * stage_bytes + r * 128;
+      const uint32_t from = own + (c & 1) * kChunkBytes, dst = tiles + stage * stage_bytes + r * 128;
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {  // 16 bytes = 8 weights; the swizzle exchanges the pieces of a row by its number mod 8
-        uint32_t v[4];
-        nibble_pairs<X>(q[c], zero[c >> 2], v);
-        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst + ((c ^ (r & 7)) << 4)),
-                     "r"(__byte_perm(v[0], v[1], 0x5410)), "r"(__byte_perm(v[2], v[3], 0x5410)),
-                     "r"(__byte_perm(v[0], v[1], 0x7632)), "r"(__byte_perm(v[2], v[3], 0x7632))
-                     : "memory");
+      for (int i = 0; i < 4; ++i) {  // 16 weights
+        const uint32_t v = (zero_bits >> (4 * ((b * kBlockK + 16 * i) / GROUP))) & 15u;
+        const uint32_t zero = nibble_magic<X>() | v | (v << 16);
+        uint32_t q[2];
+        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];"
+                     : "=r"(q[0]), "=r"(q[1])
+                     : "r"(from + (((2 * b + (i >> 1)) ^ (r & 7)) << 4) + 8 * (i & 1)));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {  // 8 weights = 16 bytes; the swizzle exchanges the pieces of a row by its number mod 8
+          uint32_t o[4];
+          nibble_pairs<X>(q[h], zero, o);
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (((2 * i + h) ^ (r & 7)) << 4)),
+                       "r"(__byte_perm(o[0], o[1], 0x5410)), "r"(__byte_perm(o[2], o[3], 0x5410)),
+                       "r"(__byte_perm(o[0], o[1], 0x7632)), "r"(__byte_perm(o[2], o[3], 0x7632))
+                       : "memory");
+        }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the tensor core reads through the async proxy
       __syncwarp();
-      if (lane == 0) mbar_arrive(full(stage));
+      if (lane == 0) {
+        mbar_arrive(full(stage));
+        if (p.wide && (b == kChunkBlocks - 1 || kb + 1 == kb1)) mbar_arrive(wempty(c & 1));
+      }
       if (++stage == p.stages) {
         stage = 0;
         phase ^= 1u;
@@ -233,19 +299,33 @@ k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ Para
     const int c0 = wg == 2 ? 0 : half, width = wg == 2 ? half : max(p.cols - half, 0);
     const int groups = static_cast<int>((p.a.k + GROUP - 1) / GROUP);
     const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + c0;
-    float sum[128];
+    uint64_t sum[64];  // pairs of columns: one instruction multiplies and adds both
 #pragma unroll
-    for (int j = 0; j < 128; ++j) sum[j] = 0.0f;
+    for (int j = 0; j < 64; ++j) sum[j] = 0;
     int acc = 0;
     uint32_t acc_phase = 0;
     const int g1 = u1 * kGroups;
     auto scale_of = [&](int g) {
       return g < groups ? load_scale(p.a.scale4, p.a.scale_type, nc * p.a.scale_stride + g) : 0.0f;
     };
-    float next = scale_of(u0 * kGroups);
-    for (int g = u0 * kGroups; g < g1; ++g) {
-      const float scale = next;
-      if (g + 1 < g1) next = scale_of(g + 1);
+    // four groups' scales are loaded four groups ahead. The loop over the groups stays rolled: the roles' hot
+    // loops together have to fit the instruction cache (unrolled by four they did not: 400 against TODO us)
+    const int g0 = u0 * kGroups;
+    float scale[4], next[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) next[i] = scale_of(g0 + i);
+#pragma unroll 1
+    for (int g = g0; g < g1; ++g) {
+      const int i = (g - g0) & 3;
+      if (i == 0) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          scale[j] = next[j];
+          next[j] = scale_of(g + 4 + j);
+        }
+      }
+      const float s = i == 0 ? scale[0] : i == 1 ? scale[1] : i == 2 ? scale[2] : scale[3];
+      const uint64_t ss = pair(__float_as_uint(s), __float_as_uint(s));
       if (!mbar_wait(tfull(acc), acc_phase, abort)) break;
       tc_fence_after();
 #pragma unroll
@@ -254,7 +334,8 @@ k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ Para
           uint32_t v[32];
           tmem_load_32(taddr + acc * p.acc_cols + c, v);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) sum[c + j] = fmaf(scale, __uint_as_float(v[j]), sum[c + j]);
+          for (int j = 0; j < 32; j += 2)
+            asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(sum[(c + j) / 2]) : "l"(pair(v[j], v[j + 1])), "l"(ss));
         }
       }
       tc_fence_before();
@@ -269,14 +350,14 @@ k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ Para
 #pragma unroll
         for (int j = 0; j < 128; ++j)
           if (j < width && t0 + c0 + j < p.a.rows)
-            store_out(p.a.out, p.a.out_type, (t0 + c0 + j) * p.a.out_stride + n, sum[j]);
+            store_out(p.a.out, p.a.out_type, (t0 + c0 + j) * p.a.out_stride + n, half_of(sum[j / 2], j & 1));
       }
     } else {
       // the ring is free: the last group's accumulator was complete, so every operand had been read
 #pragma unroll
       for (int j = 0; j < 128; ++j)
         if (j < width)
-          asm volatile("st.shared.f32 [%0], %1;" ::"r"(tiles + ((c0 + j) * kTileM + row) * 4), "f"(sum[j]) : "memory");
+          asm volatile("st.shared.f32 [%0], %1;" ::"r"(tiles + ((c0 + j) * kTileM + row) * 4), "f"(half_of(sum[j / 2], j & 1)) : "memory");
     }
     __syncwarp();
   }
@@ -286,13 +367,22 @@ k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ Para
     if (wg >= 2) {
       const int row = threadIdx.x & 127;
       if (n0 + row < p.a.n) {
-        // part r adds columns r, r + parts, ...; the two warpgroups take them in turn
-        for (int c = part + parts * (wg - 2); c < p.cols; c += 2 * parts) {
-          if (t0 + c >= p.a.rows) break;
-          const uint32_t at = tiles + (c * kTileM + row) * 4;
-          float v = 0.0f;
-          for (int r = 0; r < parts; ++r) v += __uint_as_float(load_cluster(map_to_cta(at, r)));
-          store_out(p.a.out, p.a.out_type, (t0 + c) * p.a.out_stride + n0 + row, v);
+        // part r adds columns r, r + parts, ...; the two warpgroups take eight in turn, whose remote loads overlap
+        const int last = static_cast<int>(min(static_cast<int64_t>(p.cols), p.a.rows - t0));
+        for (int c = part + 8 * parts * (wg - 2); c < last; c += 16 * parts) {
+          float v[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+          for (int r = 0; r < parts; ++r) {
+            const uint32_t base = map_to_cta(tiles + row * 4, r);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (c + j * parts < last) v[j] += __uint_as_float(load_cluster(base + (c + j * parts) * kTileM * 4));
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (c + j * parts < last)
+              store_out(p.a.out, p.a.out_type, (t0 + c + j * parts) * p.a.out_stride + n0 + row, v[j]);
         }
       }
     }
@@ -308,7 +398,7 @@ k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ Para
   }
 }
 
-using Kernel = void (*)(const CUtensorMap, const Params);
+using Kernel = void (*)(const CUtensorMap, const CUtensorMap, const Params);
 template <typename X>
 Kernel kernel_of(int group) {
   return group == 128 ? k_dense4<X, 128> : group == 64 ? k_dense4<X, 64> : k_dense4<X, 32>;
@@ -345,22 +435,26 @@ imd_status_t dense4_launch(const LinearArgs& a, cudaStream_t stream) {
   p.cols = a.rows < kTileN ? static_cast<int32_t>((a.rows + 15) / 16 * 16) : kTileN;
   p.acc_cols = 32;
   while (p.acc_cols < p.cols) p.acc_cols *= 2;
-  p.wide = reinterpret_cast<uintptr_t>(a.w) % 16 == 0 && (a.n == 1 || a.w_stride % 16 == 0);
+  p.wide = reinterpret_cast<uintptr_t>(a.w) % 16 == 0 && (a.n == 1 || (a.w_stride % 16 == 0 && a.w_stride >= (a.k + 1) / 2));
   p.error_word = dev->error_word;
   const int stage_bytes = kBytesM + p.cols * 128;
-  p.stages = (kSmem - 1024 - kCtrlBytes) / stage_bytes;
+  p.stages = (kSmem - 1024 - kCtrlBytes - 2 * kChunkBytes) / stage_bytes;
   if (p.stages > kMaxStages) p.stages = kMaxStages;
 
-  CUtensorMap map;
-  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(a.k), static_cast<cuuint64_t>(a.rows), 1};
-  const cuuint64_t pitch = static_cast<cuuint64_t>(a.x_stride) * 2;
-  const cuuint64_t strides[2] = {pitch, pitch * a.rows};
-  const cuuint32_t box[3] = {kBlockK, static_cast<cuuint32_t>(p.cols), 1};
-  const cuuint32_t elem[3] = {1, 1, 1};
-  if (reinterpret_cast<EncodeTiled>(dev->encode_tiled)(
-          &map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(a.x), dims, strides, box, elem,
-          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+  auto encode = [&](CUtensorMap* map, CUtensorMapDataType type, const void* base, int64_t cols, int64_t rows, int64_t pitch,
+                    int box_cols, int box_rows) {
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows), 1};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(pitch), static_cast<cuuint64_t>(pitch) * rows};
+    const cuuint32_t box[3] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows), 1};
+    const cuuint32_t elem[3] = {1, 1, 1};
+    return reinterpret_cast<EncodeTiled>(dev->encode_tiled)(
+               map, type, 3, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  };
+  CUtensorMap map_x, map_w{};
+  if (!encode(&map_x, CU_TENSOR_MAP_DATA_TYPE_UINT16, a.x, a.k, a.rows, 2 * a.x_stride, kBlockK, p.cols) ||
+      (p.wide && !encode(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.w, (a.k + 1) / 2, a.n,
+                         a.n == 1 ? (a.k + 31) / 32 * 16 : a.w_stride, 128, kTileM)))
     return IMD_STATUS_CUDA_ERROR;
 
   const int64_t tiles = (a.n + kTileM - 1) / kTileM * p.tiles_t;
@@ -370,7 +464,7 @@ imd_status_t dense4_launch(const LinearArgs& a, cudaStream_t stream) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned int>(tiles), static_cast<unsigned int>(parts));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = static_cast<size_t>(p.stages) * stage_bytes + 1024 + kCtrlBytes;
+  cfg.dynamicSmemBytes = static_cast<size_t>(p.stages) * stage_bytes + 2 * kChunkBytes + 1024 + kCtrlBytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -378,7 +472,7 @@ imd_status_t dense4_launch(const LinearArgs& a, cudaStream_t stream) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   const Kernel k = a.x_type == IMD_TYPE_F16 ? kernel_of<__half>(a.group) : kernel_of<__nv_bfloat16>(a.group);
-  const bool ok = cudaLaunchKernelEx(&cfg, k, map, p) == cudaSuccess;
+  const bool ok = cudaLaunchKernelEx(&cfg, k, map_x, map_w, p) == cudaSuccess;
   return cudaGetLastError() == cudaSuccess && ok ? IMD_STATUS_SUCCESS : IMD_STATUS_CUDA_ERROR;
 }
 

@@ -430,17 +430,28 @@ k_dense8_swap(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
       }
       __syncwarp();
       cluster_sync_all();
-      // part r adds columns r, r + parts, ...
+      // part r adds columns r, r + parts, ..., eight at a time so that the remote loads overlap
       if (warp >= 2 && n0 + row < p.n) {
-        for (int c = part; c < width; c += parts) {
-          if (c0 + c >= p.rows) break;
-          const uint32_t at = tiles + (c * kTileM + row) * 4;
-          uint32_t v = load_cluster(map_to_cta(at, 0));
-          for (int r = 1; r < parts; ++r) {
-            const uint32_t u = load_cluster(map_to_cta(at, r));
-            v = I8 ? v + u : __float_as_uint(__uint_as_float(v) + __uint_as_float(u));
+        const int last = min(width, p.rows - c0);
+        for (int c = part; c < last; c += 8 * parts) {
+          uint32_t v[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = 0;  // also 0.0f
+          for (int r = 0; r < parts; ++r) {
+            const uint32_t base = map_to_cta(tiles + row * 4, r);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const int cj = c + j * parts;
+              const uint32_t u = cj < last ? load_cluster(base + cj * kTileM * 4) : 0u;
+              v[j] = I8 ? v[j] + u : __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(u));
+            }
           }
-          store_out(p.out, p.out_type, (c0 + c) * p.out_stride + n0 + row, acc_value<I8>(v) * p.x_scale[c0 + c] * ws);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int cj = c0 + c + j * parts;
+            if (cj < c0 + last)
+              store_out(p.out, p.out_type, cj * p.out_stride + n0 + row, acc_value<I8>(v[j]) * p.x_scale[cj] * ws);
+          }
         }
       }
       __syncwarp();
@@ -456,7 +467,8 @@ k_dense8_swap(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
   }
 }
 
-constexpr int kSwapSmem = 200 * 1024;
+// Two CTAs of an SM take turns (one stores while the other loads) as long as their rings stay deep enough.
+constexpr int kSwapSmem = 200 * 1024, kSwapSmemHalf = 110 * 1024, kSwapColsHalf = 128;
 
 bool encode_rows(const DeviceInfo& dev, CUtensorMap* map, const void* base, int64_t k, int64_t rows, int64_t stride, int box_rows) {
   const int64_t pitch = rows > 1 ? stride : (k + 15) / 16 * 16;
@@ -499,10 +511,11 @@ bool launch_swap(const LinearArgs& a, const DeviceInfo& dev, Params p, cudaStrea
       !encode_rows(dev, &mw, a.w, a.k, a.n, a.w_stride, kTileM))
     return false;
   const int64_t tiles = (a.n + kTileM - 1) / kTileM;
+  const bool two = p.cols <= kSwapColsHalf;
   int parts = 1;  // CTAs that share a row tile: enough to occupy the SMs, at least two K blocks each
-  while (parts < 8 && tiles * parts * 2 <= dev.sms && p.k_blocks >= 4 * parts) parts *= 2;
+  while (parts < 8 && tiles * parts * 2 <= dev.sms * (two ? 2 : 1) && p.k_blocks >= 4 * parts) parts *= 2;
   const int stage_bytes = kBytesM + p.cols * kTileK;
-  p.stages = (kSwapSmem - 1024 - kCtrlBytes) / stage_bytes;
+  p.stages = ((two ? kSwapSmemHalf : kSwapSmem) - 1024 - kCtrlBytes) / stage_bytes;
   if (p.stages > kSwapMaxStages) p.stages = kSwapMaxStages;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned int>(tiles), static_cast<unsigned int>(parts));
@@ -547,7 +560,7 @@ bool dense8_takes(const LinearArgs& a) {
   auto rows_ok = [&](const void* p, int64_t rows, int64_t stride) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows == 1 || (stride % 16 == 0 && stride >= a.k));
   };
-  return a.kind != WeightKind::kU4 && a.k > 0 && a.rows > 16 && rows_ok(a.x, a.rows, a.x_stride) && rows_ok(a.w, a.n, a.w_stride);
+  return a.kind != WeightKind::kU4 && a.k > 0 && rows_ok(a.x, a.rows, a.x_stride) && rows_ok(a.w, a.n, a.w_stride);
 }
 
 imd_status_t dense8_launch(const LinearArgs& a, cudaStream_t stream) {

@@ -26,12 +26,6 @@ constexpr float kTiny = 0x1p-90f, kHuge = 0x1p+120f;
 // Row reductions. WARP: the row belongs to one warp. Otherwise to the CTA: each warp leaves its
 // partial in shared memory, one barrier, and every warp folds the partials in the same order.
 // Consecutive reductions of a row use different slots, so one barrier each is enough.
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-               "l"(src), "r"(bytes), "r"(bar)
-               : "memory");
-}
-
 template <bool WARP>
 __device__ __forceinline__ float row_sum(float v, float* slot) {
 #pragma unroll

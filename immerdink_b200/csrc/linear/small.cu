@@ -1,4 +1,5 @@
-// Products with few rows of x: the weights' bytes are the cost, each is read once.
+// Products of operands whose rows start anywhere, with any number of rows: what the kernels that move 16-byte
+// units (stream.cu, dense8.cu, dense4.cu) cannot take.
 //
 //   8 bits:  out[t, n] = xs[t] ws[n] sum_k x[t, k] w[n, k]
 //   4 bits:  out[t, n] = sum_g ws[n, g] sum_{k in g} x[t, k] (w[n, k] - z[n, g])
@@ -6,8 +7,8 @@
 // A CTA owns 16 rows of w (one mma.sync row tile) and up to 8 NT rows of x; its eight warps take the
 // K chunks in turn and their partial sums are folded in a fixed order at the end. The order of k
 // inside a chunk is free as long as both operands use the same one: a lane takes the consecutive k of
-// its quarter of the chunk with one wide load per row, and whatever four (16-bit) or eight
-// (8-bit) of them a tensor instruction wants are already in its registers.
+// its quarter of the chunk, and whatever four (16-bit) or eight (8-bit) of them a tensor instruction
+// wants are already in its registers.
 //
 // 4-bit weights become exact 16-bit floats: a nibble or'ed into the mantissa of 128 (bf16) or 1024
 // (f16) is 128 + w or 1024 + w, and subtracting 128 + z or 1024 + z is exact. A shift by 4 i and one
@@ -16,6 +17,7 @@
 // e4m3 values are exact in f16 and their products are summed in 32-bit floats by the f16 instruction.
 #include <cstdint>
 
+#include "mma.cuh"
 #include "types.cuh"
 
 namespace imd {
@@ -23,35 +25,6 @@ namespace {
 
 constexpr int kWarps = 8;
 constexpr int kRowsPerTile = 16;
-
-__device__ __forceinline__ void mma_f16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-      "{%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma_bf16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-      "{%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma_s8(int* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-      "{%0, %1, %2, %3};"
-      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ void mma_pair(float* d, const uint32_t* a, uint32_t b0, uint32_t b1, __half) {
-  mma_f16(d, a, b0, b1);
-}
-__device__ __forceinline__ void mma_pair(float* d, const uint32_t* a, uint32_t b0, uint32_t b1, __nv_bfloat16) {
-  mma_bf16(d, a, b0, b1);
-}
 
 // Folds the warps' partial tiles in the order of the warps and hands each output to `write`.
 template <int NT, typename Acc, typename Write>
@@ -73,7 +46,7 @@ __device__ __forceinline__ void fold(Acc (*acc)[4], const LinearArgs& p, int64_t
   }
 }
 
-template <typename X, int GROUP, int NT, bool WIDE>
+template <typename X, int GROUP, int NT>
 __global__ void __launch_bounds__(32 * kWarps) k_small_w4(const __grid_constant__ LinearArgs p) {
   constexpr int kBytes = GROUP / 8;       // weights of one lane and row in one group
   constexpr int kWords = kBytes / 4;
@@ -93,7 +66,7 @@ __global__ void __launch_bounds__(32 * kWarps) k_small_w4(const __grid_constant_
     float scale[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      load_bytes<kBytes, WIDE>(w[h], k0 / 2, w_end, span_w, q[h]);
+      load_bytes<kBytes>(w[h], k0 / 2, w_end, span_w, q[h]);
       scale[h] = load_scale(p.scale4, p.scale_type, row[h] * p.scale_stride + g);
       const uint32_t z = p.zeros == nullptr ? 8u : p.zeros[row[h] * p.zeros_stride + g] & 15u;
       zero[h] = kMagic | z | (z << 16);
@@ -103,7 +76,7 @@ __global__ void __launch_bounds__(32 * kWarps) k_small_w4(const __grid_constant_
     for (int j = 0; j < NT; ++j) {
       const int64_t t = t0 + 8 * j + (lane >> 2);
       if (t < p.rows) {
-        load_bytes<16 * kWords, WIDE>(static_cast<const uint8_t*>(p.x) + 2 * t * p.x_stride, 2 * k0, 2 * p.k, span_x, &x[j][0][0]);
+        load_bytes<16 * kWords>(static_cast<const uint8_t*>(p.x) + 2 * t * p.x_stride, 2 * k0, 2 * p.k, span_x, &x[j][0][0]);
       } else {
 #pragma unroll
         for (int i = 0; i < 4 * kWords; ++i) (&x[j][0][0])[i] = 0;
@@ -131,18 +104,7 @@ __global__ void __launch_bounds__(32 * kWarps) k_small_w4(const __grid_constant_
   fold<NT, float>(acc, p, n0, t0, [&](int64_t t, int64_t n, float v) { store_out(p.out, p.out_type, t * p.out_stride + n, v); });
 }
 
-// 16 e4m3 values (4 words) as f16 pairs.
-__device__ __forceinline__ void widen(const uint32_t* q, uint32_t (*h)[2]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(q[i] >> (16 * b)), __NV_E4M3);
-      h[i][b] = static_cast<uint32_t>(r.x) | (static_cast<uint32_t>(r.y) << 16);
-    }
-}
-
-template <bool I8, int NT, bool WIDE>
+template <bool I8, int NT>
 __global__ void __launch_bounds__(32 * kWarps) k_small_8(const __grid_constant__ LinearArgs p) {
   using Acc = typename std::conditional<I8, int, float>::type;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -157,12 +119,12 @@ __global__ void __launch_bounds__(32 * kWarps) k_small_8(const __grid_constant__
     const int64_t k0 = c * 64 + (lane & 3) * 16;
     uint32_t q[2][4], x[NT][4];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) load_bytes<16, WIDE>(w[h], k0, p.k, span_w, q[h]);
+    for (int h = 0; h < 2; ++h) load_bytes<16>(w[h], k0, p.k, span_w, q[h]);
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       const int64_t t = t0 + 8 * j + (lane >> 2);
       if (t < p.rows) {
-        load_bytes<16, WIDE>(static_cast<const uint8_t*>(p.x) + t * p.x_stride, k0, p.k, span_x, x[j]);
+        load_bytes<16>(static_cast<const uint8_t*>(p.x) + t * p.x_stride, k0, p.k, span_x, x[j]);
       } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[j][i] = 0;
@@ -178,9 +140,9 @@ __global__ void __launch_bounds__(32 * kWarps) k_small_8(const __grid_constant__
     } else {
       uint32_t wide[2][4][2], wx[NT][4][2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) widen(q[h], wide[h]);
+      for (int h = 0; h < 2; ++h) widen_e4m3(q[h], wide[h]);
 #pragma unroll
-      for (int j = 0; j < NT; ++j) widen(x[j], wx[j]);
+      for (int j = 0; j < NT; ++j) widen_e4m3(x[j], wx[j]);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint32_t a[4] = {wide[0][i][0], wide[1][i][0], wide[0][i][1], wide[1][i][1]};
@@ -194,25 +156,21 @@ __global__ void __launch_bounds__(32 * kWarps) k_small_8(const __grid_constant__
   });
 }
 
-bool rows_aligned(const void* p, int64_t stride_bytes, int64_t rows, int unit) {
-  return reinterpret_cast<uintptr_t>(p) % unit == 0 && (rows <= 1 || stride_bytes % unit == 0);
-}
-
-template <int NT, bool WIDE>
+template <int NT>
 void launch(const LinearArgs& a, dim3 grid, cudaStream_t stream) {
   constexpr int threads = 32 * kWarps;
   if (a.kind == WeightKind::kI8) {
-    k_small_8<true, NT, WIDE><<<grid, threads, 0, stream>>>(a);
+    k_small_8<true, NT><<<grid, threads, 0, stream>>>(a);
   } else if (a.kind == WeightKind::kE4M3) {
-    k_small_8<false, NT, WIDE><<<grid, threads, 0, stream>>>(a);
+    k_small_8<false, NT><<<grid, threads, 0, stream>>>(a);
   } else if (a.x_type == IMD_TYPE_F16) {
-    if (a.group == 128) k_small_w4<__half, 128, NT, WIDE><<<grid, threads, 0, stream>>>(a);
-    else if (a.group == 64) k_small_w4<__half, 64, NT, WIDE><<<grid, threads, 0, stream>>>(a);
-    else k_small_w4<__half, 32, NT, WIDE><<<grid, threads, 0, stream>>>(a);
+    if (a.group == 128) k_small_w4<__half, 128, NT><<<grid, threads, 0, stream>>>(a);
+    else if (a.group == 64) k_small_w4<__half, 64, NT><<<grid, threads, 0, stream>>>(a);
+    else k_small_w4<__half, 32, NT><<<grid, threads, 0, stream>>>(a);
   } else {
-    if (a.group == 128) k_small_w4<__nv_bfloat16, 128, NT, WIDE><<<grid, threads, 0, stream>>>(a);
-    else if (a.group == 64) k_small_w4<__nv_bfloat16, 64, NT, WIDE><<<grid, threads, 0, stream>>>(a);
-    else k_small_w4<__nv_bfloat16, 32, NT, WIDE><<<grid, threads, 0, stream>>>(a);
+    if (a.group == 128) k_small_w4<__nv_bfloat16, 128, NT><<<grid, threads, 0, stream>>>(a);
+    else if (a.group == 64) k_small_w4<__nv_bfloat16, 64, NT><<<grid, threads, 0, stream>>>(a);
+    else k_small_w4<__nv_bfloat16, 32, NT><<<grid, threads, 0, stream>>>(a);
   }
 }
 
@@ -220,8 +178,6 @@ void launch(const LinearArgs& a, dim3 grid, cudaStream_t stream) {
 
 imd_status_t linear_small_launch(const LinearArgs& a, cudaStream_t stream) {
   const int x_size = a.kind == WeightKind::kU4 ? 2 : 1;
-  const int w_unit = a.kind == WeightKind::kU4 ? a.group / 8 : 16;
-  const bool wide = rows_aligned(a.x, a.x_stride * x_size, a.rows, 16) && rows_aligned(a.w, a.w_stride, a.n, w_unit);
   const int nt = a.rows <= 8 ? 1 : a.rows <= 16 ? 2 : 4;
   const int64_t tiles = (a.rows + 8 * nt - 1) / (8 * nt);
   LinearArgs part = a;
@@ -232,9 +188,9 @@ imd_status_t linear_small_launch(const LinearArgs& a, cudaStream_t stream) {
     if (a.x_scale != nullptr) part.x_scale = a.x_scale + t0;
     part.out = static_cast<uint8_t*>(a.out) + t0 * a.out_stride * (a.out_type == IMD_TYPE_F32 ? 4 : 2);
     const dim3 grid(static_cast<unsigned int>((a.n + kRowsPerTile - 1) / kRowsPerTile), static_cast<unsigned int>(count));
-    if (nt == 1) wide ? launch<1, true>(part, grid, stream) : launch<1, false>(part, grid, stream);
-    else if (nt == 2) wide ? launch<2, true>(part, grid, stream) : launch<2, false>(part, grid, stream);
-    else wide ? launch<4, true>(part, grid, stream) : launch<4, false>(part, grid, stream);
+    if (nt == 1) launch<1>(part, grid, stream);
+    else if (nt == 2) launch<2>(part, grid, stream);
+    else launch<4>(part, grid, stream);
   }
   return cudaGetLastError() == cudaSuccess ? IMD_STATUS_SUCCESS : IMD_STATUS_CUDA_ERROR;
 }

@@ -51,41 +51,24 @@ __device__ __forceinline__ Span span_of(const void* p, int64_t rows, int64_t str
   return {lo, lo + static_cast<uintptr_t>((rows - 1) * stride_bytes + row_bytes)};
 }
 
-// `BYTES` bytes at row + at, zeros from `end` (the row's length in bytes) on. WIDE: row + at is aligned to
-// min(BYTES, 16). Rows of any alignment are read as the aligned words around them, shifted into place,
-// wherever those words lie inside the matrix; single bytes remain at its two ends and at a row's end.
-template <int BYTES, bool WIDE>
+// `BYTES` bytes at row + at, zeros from `end` (the row's length in bytes) on, for rows of any alignment: they
+// are read as the aligned words around them, shifted into place, wherever those words lie inside the matrix;
+// single bytes remain at its two ends and at a row's end.
+template <int BYTES>
 __device__ __forceinline__ void load_bytes(const uint8_t* row, int64_t at, int64_t end, const Span& span, uint32_t* v) {
   const uint8_t* p = row + at;
-  if (at + BYTES <= end) {
-    if (WIDE) {
-      if constexpr (BYTES >= 16) {
+  const uintptr_t first = reinterpret_cast<uintptr_t>(p) & ~static_cast<uintptr_t>(3);
+  if (at + BYTES <= end && first >= span.lo && first + BYTES + 4 <= span.hi) {
+    const uint32_t shift = 8 * (reinterpret_cast<uintptr_t>(p) & 3);
+    const uint32_t* q = reinterpret_cast<const uint32_t*>(first);
+    uint32_t low = q[0];
 #pragma unroll
-        for (int i = 0; i < BYTES / 4; i += 4) {
-          const uint4 t = *reinterpret_cast<const uint4*>(p + 4 * i);
-          v[i] = t.x, v[i + 1] = t.y, v[i + 2] = t.z, v[i + 3] = t.w;
-        }
-      } else if constexpr (BYTES == 8) {
-        const uint2 t = *reinterpret_cast<const uint2*>(p);
-        v[0] = t.x, v[1] = t.y;
-      } else {
-        v[0] = *reinterpret_cast<const uint32_t*>(p);
-      }
-      return;
+    for (int i = 0; i < BYTES / 4; ++i) {
+      const uint32_t high = q[i + 1];
+      v[i] = __funnelshift_r(low, high, shift);
+      low = high;
     }
-    const uintptr_t first = reinterpret_cast<uintptr_t>(p) & ~static_cast<uintptr_t>(3);
-    if (first >= span.lo && first + BYTES + 4 <= span.hi) {
-      const uint32_t shift = 8 * (reinterpret_cast<uintptr_t>(p) & 3);
-      const uint32_t* q = reinterpret_cast<const uint32_t*>(first);
-      uint32_t low = q[0];
-#pragma unroll
-      for (int i = 0; i < BYTES / 4; ++i) {
-        const uint32_t high = q[i + 1];
-        v[i] = __funnelshift_r(low, high, shift);
-        low = high;
-      }
-      return;
-    }
+    return;
   }
 #pragma unroll
   for (int i = 0; i < BYTES / 4; ++i) {
