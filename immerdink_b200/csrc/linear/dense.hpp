@@ -1,5 +1,7 @@
 // The tensor-core kernels' share of a device: what is looked up or set once per device.
 #pragma once
+#include <cuda.h>
+
 #include "linear.hpp"
 
 namespace imd {
@@ -11,6 +13,14 @@ struct DeviceInfo {
 };
 // Of the current device; made on first use, nullptr where that fails (asked again at the next call).
 const DeviceInfo* device_info();
+
+// Rows that TMA can bring: 16-byte units, not overlapping.
+inline bool rows_for_tma(const void* p, int64_t rows, int64_t stride_bytes, int64_t row_bytes) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows == 1 || (stride_bytes % 16 == 0 && stride_bytes >= row_bytes));
+}
+// Tensor map of such rows as bytes, boxes of box_rows x 128 bytes with the 128-byte swizzle; what lies outside is zero.
+bool encode_rows_128(const DeviceInfo& dev, CUtensorMap* map, const void* base, int64_t row_bytes, int64_t rows,
+                     int64_t stride_bytes, int box_rows);
 
 bool norm_setup();  // kernel attributes on the current device
 // The same; whether these kernels take this call; the call.

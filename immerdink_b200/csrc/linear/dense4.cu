@@ -141,7 +141,7 @@ k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUte
           break;
         }
         mbar_expect_tx(full(stage), p.cols * 128);
-        tma_load_3d(tiles + stage * stage_bytes + kBytesM, &map_x, full(stage), kb * kBlockK, static_cast<int>(t0), 0, policy);
+        tma_load_3d(tiles + stage * stage_bytes + kBytesM, &map_x, full(stage), kb * 2 * kBlockK, static_cast<int>(t0), 0, policy);
         issued |= 1u << stage;
         if (++stage == p.stages) {
           stage = 0;
@@ -420,8 +420,7 @@ bool dense4_setup() {
 }
 
 bool dense4_takes(const LinearArgs& a) {
-  return a.kind == WeightKind::kU4 && a.k > 0 && a.rows > 16 && reinterpret_cast<uintptr_t>(a.x) % 16 == 0 &&
-         a.x_stride % 8 == 0 && a.x_stride >= a.k;
+  return a.kind == WeightKind::kU4 && a.k > 0 && a.rows > 16 && rows_for_tma(a.x, a.rows, 2 * a.x_stride, 2 * a.k);
 }
 
 imd_status_t dense4_launch(const LinearArgs& a, cudaStream_t stream) {
@@ -435,26 +434,16 @@ imd_status_t dense4_launch(const LinearArgs& a, cudaStream_t stream) {
   p.cols = a.rows < kTileN ? static_cast<int32_t>((a.rows + 15) / 16 * 16) : kTileN;
   p.acc_cols = 32;
   while (p.acc_cols < p.cols) p.acc_cols *= 2;
-  p.wide = reinterpret_cast<uintptr_t>(a.w) % 16 == 0 && (a.n == 1 || (a.w_stride % 16 == 0 && a.w_stride >= (a.k + 1) / 2));
+  p.wide = rows_for_tma(a.w, a.n, a.w_stride, (a.k + 1) / 2);
   p.error_word = dev->error_word;
   const int stage_bytes = kBytesM + p.cols * 128;
   p.stages = (kSmem - 1024 - kCtrlBytes - 2 * kChunkBytes) / stage_bytes;
   if (p.stages > kMaxStages) p.stages = kMaxStages;
 
-  auto encode = [&](CUtensorMap* map, CUtensorMapDataType type, const void* base, int64_t cols, int64_t rows, int64_t pitch,
-                    int box_cols, int box_rows) {
-    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows), 1};
-    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(pitch), static_cast<cuuint64_t>(pitch) * rows};
-    const cuuint32_t box[3] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows), 1};
-    const cuuint32_t elem[3] = {1, 1, 1};
-    return reinterpret_cast<EncodeTiled>(dev->encode_tiled)(
-               map, type, 3, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-  };
+  // the swizzle goes by bytes, so x is described as bytes too
   CUtensorMap map_x, map_w{};
-  if (!encode(&map_x, CU_TENSOR_MAP_DATA_TYPE_UINT16, a.x, a.k, a.rows, 2 * a.x_stride, kBlockK, p.cols) ||
-      (p.wide && !encode(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.w, (a.k + 1) / 2, a.n,
-                         a.n == 1 ? (a.k + 31) / 32 * 16 : a.w_stride, 128, kTileM)))
+  if (!encode_rows_128(*dev, &map_x, a.x, 2 * a.k, a.rows, 2 * a.x_stride, p.cols) ||
+      (p.wide && !encode_rows_128(*dev, &map_w, a.w, (a.k + 1) / 2, a.n, a.w_stride, kTileM)))
     return IMD_STATUS_CUDA_ERROR;
 
   const int64_t tiles = (a.n + kTileM - 1) / kTileM * p.tiles_t;

@@ -470,23 +470,11 @@ k_dense8_swap(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
 // Two CTAs of an SM take turns (one stores while the other loads) as long as their rings stay deep enough.
 constexpr int kSwapSmem = 200 * 1024, kSwapSmemHalf = 110 * 1024, kSwapColsHalf = 128;
 
-bool encode_rows(const DeviceInfo& dev, CUtensorMap* map, const void* base, int64_t k, int64_t rows, int64_t stride, int box_rows) {
-  const int64_t pitch = rows > 1 ? stride : (k + 15) / 16 * 16;
-  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rows), 1};
-  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(pitch), static_cast<cuuint64_t>(pitch) * rows};
-  const cuuint32_t box[3] = {kTileK, static_cast<cuuint32_t>(box_rows), 1};
-  const cuuint32_t elem[3] = {1, 1, 1};
-  const EncodeTiled fn = reinterpret_cast<EncodeTiled>(dev.encode_tiled);
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, elem,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <bool I8, int BN>
 bool launch_pair(const LinearArgs& a, const DeviceInfo& dev, Params p, cudaStream_t stream) {
   CUtensorMap mx, mw;
-  if (!encode_rows(dev, &mx, a.x, a.k, a.rows, a.x_stride, 128) ||
-      !encode_rows(dev, &mw, a.w, a.k, a.n, a.w_stride, BN / 2))
+  if (!encode_rows_128(dev, &mx, a.x, a.k, a.rows, a.x_stride, 128) ||
+      !encode_rows_128(dev, &mw, a.w, a.k, a.n, a.w_stride, BN / 2))
     return false;
   p.tiles_m = static_cast<int32_t>((a.rows + 255) / 256);
   p.tiles_n = static_cast<int32_t>((a.n + BN - 1) / BN);
@@ -507,8 +495,8 @@ bool launch_swap(const LinearArgs& a, const DeviceInfo& dev, Params p, cudaStrea
   p.cols = static_cast<int32_t>((a.rows + 15) / 16 * 16);
   p.tmem_cols = 32;
   while (p.tmem_cols < p.cols) p.tmem_cols *= 2;
-  if (!encode_rows(dev, &mx, a.x, a.k, a.rows, a.x_stride, p.cols) ||
-      !encode_rows(dev, &mw, a.w, a.k, a.n, a.w_stride, kTileM))
+  if (!encode_rows_128(dev, &mx, a.x, a.k, a.rows, a.x_stride, p.cols) ||
+      !encode_rows_128(dev, &mw, a.w, a.k, a.n, a.w_stride, kTileM))
     return false;
   const int64_t tiles = (a.n + kTileM - 1) / kTileM;
   const bool two = p.cols <= kSwapColsHalf;
@@ -555,12 +543,8 @@ bool launch(const LinearArgs& a, const DeviceInfo& dev, const Params& p, cudaStr
 
 bool dense8_setup() { return set_attributes<true>() && set_attributes<false>(); }
 
-// TMA wants 16-byte rows; a matrix whose rows overlap (a repeated row) stays with the small kernel.
 bool dense8_takes(const LinearArgs& a) {
-  auto rows_ok = [&](const void* p, int64_t rows, int64_t stride) {
-    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows == 1 || (stride % 16 == 0 && stride >= a.k));
-  };
-  return a.kind != WeightKind::kU4 && a.k > 0 && rows_ok(a.x, a.rows, a.x_stride) && rows_ok(a.w, a.n, a.w_stride);
+  return a.kind != WeightKind::kU4 && a.k > 0 && rows_for_tma(a.x, a.rows, a.x_stride, a.k) && rows_for_tma(a.w, a.n, a.w_stride, a.k);
 }
 
 imd_status_t dense8_launch(const LinearArgs& a, cudaStream_t stream) {

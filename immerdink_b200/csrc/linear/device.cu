@@ -2,6 +2,7 @@
 // waits, the SM count and the kernels' shared-memory attributes. Made once per device, never changed.
 #include <mutex>
 
+#include "cuda/sm100.cuh"
 #include "dense.hpp"
 
 namespace imd {
@@ -29,6 +30,19 @@ bool make(int device, DeviceInfo* info) {
 }
 
 }  // namespace
+
+bool encode_rows_128(const DeviceInfo& dev, CUtensorMap* map, const void* base, int64_t row_bytes, int64_t rows,
+                     int64_t stride_bytes, int box_rows) {
+  const int64_t pitch = rows > 1 ? stride_bytes : (row_bytes + 15) / 16 * 16;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(row_bytes), static_cast<cuuint64_t>(rows), 1};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(pitch), static_cast<cuuint64_t>(pitch) * rows};
+  const cuuint32_t box[3] = {128, static_cast<cuuint32_t>(box_rows), 1};
+  const cuuint32_t elem[3] = {1, 1, 1};
+  const EncodeTiled fn = reinterpret_cast<EncodeTiled>(dev.encode_tiled);
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, elem,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 
 const DeviceInfo* device_info() {
   int device = 0;
