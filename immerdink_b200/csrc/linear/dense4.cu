@@ -64,15 +64,6 @@ __device__ __forceinline__ uint32_t load_cluster(uint32_t addr) {
   return v;
 }
 
-__device__ __forceinline__ uint64_t pair(uint32_t lo, uint32_t hi) {
-  uint64_t v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
-  return v;
-}
-__device__ __forceinline__ float half_of(uint64_t v, int high) {
-  return __uint_as_float(static_cast<uint32_t>(high != 0 ? v >> 32 : v));
-}
-
 template <typename X, int GROUP>
 __global__ void __launch_bounds__(kThreads, 1)
 k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
@@ -165,9 +156,8 @@ k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUte
         if (!mbar_wait(full(stage), phase, abort)) break;
         tc_fence_after();
         const uint32_t a = tiles + stage * stage_bytes, b = a + kBytesM;
-        uint64_t da = smem_desc(a), db = smem_desc(b);
 #pragma unroll
-        for (int i = 0; i < 4; ++i, da += 2, db += 2) {  // 16 k = 32 bytes an instruction
+        for (int i = 0; i < 4; ++i) {  // 16 k = 32 bytes an instruction
           const int at = (kb % kBlocks) * kBlockK + 16 * i;  // place in the unit
           if (at % GROUP == 0) {
             if (!mbar_wait(tempty(acc), acc_phase ^ 1u, abort)) {
@@ -176,7 +166,7 @@ k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUte
             }
             tc_fence_after();
           }
-          mma16<X>(tmem_base + acc * p.acc_cols, da, db, idesc, at % GROUP != 0);
+          mma16<X>(tmem_base + acc * p.acc_cols, smem_desc(a + 32 * i), smem_desc(b + 32 * i), idesc, at % GROUP != 0);
           if ((at + 16) % GROUP == 0) {
             tc_commit(tfull(acc));
             acc ^= 1;
@@ -259,25 +249,28 @@ k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUte
         }
         if (p.wide && !mbar_wait(wfull(c & 1), (c >> 1) & 1, abort)) break;
       }
-      if (!mbar_wait(empty(stage), phase ^ 1u, abort)) break;
       const uint32_t from = own + (c & 1) * kChunkBytes, dst = tiles + stage * stage_bytes + r * 128;
+      uint32_t q[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {  // 16 weights
-        const uint32_t v = (zero_bits >> (4 * ((b * kBlockK + 16 * i) / GROUP))) & 15u;
-        const uint32_t zero = nibble_magic<X>() | v | (v << 16);
-        uint32_t q[2];
-        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];"
-                     : "=r"(q[0]), "=r"(q[1])
-                     : "r"(from + (((2 * b + (i >> 1)) ^ (r & 7)) << 4) + 8 * (i & 1)));
+      for (int i = 0; i < 8; i += 4)
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(q[i]), "=r"(q[i + 1]), "=r"(q[i + 2]), "=r"(q[i + 3])
+                     : "r"(from + (((2 * b + i / 4) ^ (r & 7)) << 4)));
+      uint32_t zero[2];  // of the first and the second 32 k
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {  // 8 weights = 16 bytes; the swizzle exchanges the pieces of a row by its number mod 8
-          uint32_t o[4];
-          nibble_pairs<X>(q[h], zero, o);
-          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (((2 * i + h) ^ (r & 7)) << 4)),
-                       "r"(__byte_perm(o[0], o[1], 0x5410)), "r"(__byte_perm(o[2], o[3], 0x5410)),
-                       "r"(__byte_perm(o[0], o[1], 0x7632)), "r"(__byte_perm(o[2], o[3], 0x7632))
-                       : "memory");
-        }
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t v = (zero_bits >> (4 * ((b * kBlockK + 32 * h) / GROUP))) & 15u;
+        zero[h] = nibble_magic<X>() | v | (v << 16);
+      }
+      if (!mbar_wait(empty(stage), phase ^ 1u, abort)) break;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {  // 16 bytes = 8 weights; the swizzle exchanges the pieces of a row by its number mod 8
+        uint32_t o[4];
+        nibble_pairs<X>(q[i], zero[i >> 2], o);
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst + ((i ^ (r & 7)) << 4)),
+                     "r"(__byte_perm(o[0], o[1], 0x5410)), "r"(__byte_perm(o[2], o[3], 0x5410)),
+                     "r"(__byte_perm(o[0], o[1], 0x7632)), "r"(__byte_perm(o[2], o[3], 0x7632))
+                     : "memory");
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the tensor core reads through the async proxy
       __syncwarp();
@@ -299,9 +292,9 @@ k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUte
     const int c0 = wg == 2 ? 0 : half, width = wg == 2 ? half : max(p.cols - half, 0);
     const int groups = static_cast<int>((p.a.k + GROUP - 1) / GROUP);
     const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + c0;
-    uint64_t sum[64];  // pairs of columns: one instruction multiplies and adds both
+    float sum[128];
 #pragma unroll
-    for (int j = 0; j < 64; ++j) sum[j] = 0;
+    for (int j = 0; j < 128; ++j) sum[j] = 0.0f;
     int acc = 0;
     uint32_t acc_phase = 0;
     const int g1 = u1 * kGroups;
@@ -325,7 +318,6 @@ k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUte
         }
       }
       const float s = i == 0 ? scale[0] : i == 1 ? scale[1] : i == 2 ? scale[2] : scale[3];
-      const uint64_t ss = pair(__float_as_uint(s), __float_as_uint(s));
       if (!mbar_wait(tfull(acc), acc_phase, abort)) break;
       tc_fence_after();
 #pragma unroll
@@ -334,8 +326,7 @@ k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUte
           uint32_t v[32];
           tmem_load_32(taddr + acc * p.acc_cols + c, v);
 #pragma unroll
-          for (int j = 0; j < 32; j += 2)
-            asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(sum[(c + j) / 2]) : "l"(pair(v[j], v[j + 1])), "l"(ss));
+          for (int j = 0; j < 32; ++j) sum[c + j] = fmaf(s, __uint_as_float(v[j]), sum[c + j]);
         }
       }
       tc_fence_before();
@@ -350,14 +341,14 @@ k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUte
 #pragma unroll
         for (int j = 0; j < 128; ++j)
           if (j < width && t0 + c0 + j < p.a.rows)
-            store_out(p.a.out, p.a.out_type, (t0 + c0 + j) * p.a.out_stride + n, half_of(sum[j / 2], j & 1));
+            store_out(p.a.out, p.a.out_type, (t0 + c0 + j) * p.a.out_stride + n, sum[j]);
       }
     } else {
       // the ring is free: the last group's accumulator was complete, so every operand had been read
 #pragma unroll
       for (int j = 0; j < 128; ++j)
         if (j < width)
-          asm volatile("st.shared.f32 [%0], %1;" ::"r"(tiles + ((c0 + j) * kTileM + row) * 4), "f"(half_of(sum[j / 2], j & 1)) : "memory");
+          asm volatile("st.shared.f32 [%0], %1;" ::"r"(tiles + ((c0 + j) * kTileM + row) * 4), "f"(sum[j]) : "memory");
     }
     __syncwarp();
   }

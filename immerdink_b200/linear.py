@@ -52,10 +52,10 @@ class Library:
         for name, args in SIGNATURES.items():
             f = getattr(self.lib, name)
             f.restype, f.argtypes = C.c_int, args
-        self._cudart = None
+        self._local, self._get_device = threading.local(), None
         for name in ("libcudart.so.12", "libcudart.so.13", "libcudart.so"):
             try:
-                self._cudart = C.CDLL(name)
+                self._get_device = C.CDLL(name).cudaGetDevice
                 break
             except OSError:
                 continue
@@ -70,10 +70,15 @@ class Library:
 
     def current_device(self):
         """The current device's number; None where the runtime cannot be asked."""
-        d = C.c_int(0)
-        if self._cudart is None or self._cudart.cudaGetDevice(C.byref(d)) != 0:
+        try:
+            number, ref = self._local.device
+        except AttributeError:   # this thread's first question
+            number = C.c_int(0)
+            ref = C.byref(number)
+            self._local.device = number, ref
+        if self._get_device is None or self._get_device(ref) != 0:
             return None
-        return d.value
+        return number.value
 
 
 _loaded, _lock = {}, threading.Lock()
@@ -91,7 +96,7 @@ def load_library(path=None):
     return lib
 
 
-_torch_types = {}   # torch dtype object -> code (None: not one of ours)
+_torch_types = {}   # dtype object of PyTorch -> type (None: not one of ours)
 
 
 def _view(x, what, stream, device):
@@ -122,6 +127,15 @@ def _view(x, what, stream, device):
 
 def _matrix(x, what, types, stream, device, out=False):
     """(pointer, rows, columns, row stride, type) of a matrix whose rows have unit stride."""
+    # the usual case in the fewest steps: a call costs as much on the host as on the GPU at one row
+    kind = _torch_types.get(getattr(x, "dtype", None))
+    if kind in types and x.get_device() == device:
+        shape = x.shape
+        if len(shape) == 2:
+            rows, cols = shape
+            strides = x.stride()
+            if strides[1] == 1:
+                return x.data_ptr(), rows, cols, strides[0], kind
     ptr, shape, strides, kind, readonly = _view(x, what, stream, device)
     if kind not in types:
         raise TypeError(f"{what}: dtype must be {' or '.join(_NAMES[t] for t in types)}")
@@ -139,6 +153,9 @@ def _matrix(x, what, types, stream, device, out=False):
 
 def _vector(x, what, n, types, stream, device, out=False):
     """(pointer, type) of a contiguous vector of n elements."""
+    kind = _torch_types.get(getattr(x, "dtype", None))
+    if kind in types and x.get_device() == device and x.shape == (n,) and x.stride(0) == 1:
+        return x.data_ptr(), kind
     ptr, shape, strides, kind, readonly = _view(x, what, stream, device)
     if kind not in types:
         raise TypeError(f"{what}: dtype must be {' or '.join(_NAMES[t] for t in types)}")
@@ -171,17 +188,20 @@ def norm_quantize(x, weight, q, scale, *, eps=1e-6, residual=None, residual_out=
     px, rows, dim, sx, tx = _matrix(x, "x", (F32, BF16, F16), s, dev)
     pw, tw = _vector(weight, "weight", dim, (tx, F32) if tx != F32 else (F32,), s, dev)
     pq, qr, qc, sq, tq = _matrix(q, "q", (I8, E4M3), s, dev, True)
-    _same("q", (qr, qc), (rows, dim))
+    if qr != rows or qc != dim:
+        _same("q", (qr, qc), (rows, dim))
     ps, _ = _vector(scale, "scale", rows, (F32,), s, dev, True)
     pr = sr = ph = sh = 0
     if residual is not None:
         pr, r, c, sr, _ = _matrix(residual, "residual", (tx,), s, dev)
-        _same("residual", (r, c), (rows, dim))
+        if r != rows or c != dim:
+            _same("residual", (r, c), (rows, dim))
     if residual_out is not None:
         if residual is None:
             raise ValueError("residual_out is given without a residual")
         ph, r, c, sh, _ = _matrix(residual_out, "residual_out", (tx,), s, dev, True)
-        _same("residual_out", (r, c), (rows, dim))
+        if r != rows or c != dim:
+            _same("residual_out", (r, c), (rows, dim))
     st = lib.lib.imd_norm_quantize(rows, dim, tx, px, sx, pr, sr, tw, pw, eps, ph, sh, tq, pq, sq, ps, s)
     if st:
         raise _error(st, "imd_norm_quantize")
