@@ -4,6 +4,7 @@
     libimmerdink.so        C ABI + sm_100a kernels       (nvcc -gencode arch=compute_100a,code=sm_100a)
     libimmerdink_hooks.so  the same objects + the imd_test_* / imd_prof_* entry points (tests, phase timing)
     libimmerdink_linear.so C ABI + sm_100a kernels of the quantised linear layer (nvcc)
+    _fastcall.so           its front end's host side for PyTorch tensors (g++'s C, Python.h)
 
     python -m immerdink_b200.build [--force]
 
@@ -13,6 +14,7 @@ import concurrent.futures
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -21,6 +23,7 @@ INCLUDE = os.path.join(ROOT, "include")
 HOST_LIB = os.path.join(HERE, "libimmerdink_host.so")
 CUDA_LIB = os.path.join(HERE, "libimmerdink.so")
 HOOKS_LIB = os.path.join(HERE, "libimmerdink_hooks.so")
+FASTCALL_LIB = os.path.join(HERE, "_fastcall.so")
 LINEAR_LIB = os.path.join(HERE, "libimmerdink_linear.so")
 OBJ_DIR = os.path.join(HERE, "build")
 
@@ -129,10 +132,19 @@ def build_linear(force=False, verbose=False):
     return LINEAR_LIB
 
 
+def build_fastcall(force=False):
+    src = os.path.join(CSRC, "linear", "fastcall.c")
+    if force or not os.path.exists(FASTCALL_LIB) or os.path.getmtime(FASTCALL_LIB) < os.path.getmtime(src):
+        _run([_cxx(), "-x", "c", "-std=gnu11", "-O2", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall",
+              "-I" + sysconfig.get_paths()["include"], src, "-o", FASTCALL_LIB])
+    return FASTCALL_LIB
+
+
 def build_all(force=False, verbose=False):
     build_host(force)
     build_cuda(force, verbose)
     build_linear(force, verbose)
+    build_fastcall(force)
 
 
 if __name__ == "__main__":
@@ -141,3 +153,4 @@ if __name__ == "__main__":
     print(CUDA_LIB)
     print(HOOKS_LIB)
     print(LINEAR_LIB)
+    print(FASTCALL_LIB)

@@ -10,7 +10,10 @@ stream), so it can be captured in a CUDA graph. The caller owns every array. Arr
 tensors, DLPack producers or `__cuda_array_interface__` objects; bfloat16 and float8_e4m3fn need
 one of the first two. They must be on the current device, and rows must have unit stride.
 
-There is no fallback: when the library is missing, the first call raises OSError."""
+Calls with PyTorch tensors take a short way (csrc/linear/fastcall.c) that does the same checks in C; what
+it does not take, and everything that is refused, goes through the general path below.
+
+There is no fallback: when a library is missing, the first call raises OSError."""
 import ctypes as C
 import os
 import threading
@@ -52,6 +55,12 @@ class Library:
         for name, args in SIGNATURES.items():
             f = getattr(self.lib, name)
             f.restype, f.argtypes = C.c_int, args
+        try:
+            from . import _fastcall
+        except ImportError as exc:
+            raise OSError("_fastcall.so not found (build it with `python -m immerdink_b200.build`)") from exc
+        self.fast = _fastcall
+        self._address = {name: C.cast(getattr(self.lib, name), C.c_void_p).value for name in SIGNATURES}
         self._local, self._get_device = threading.local(), None
         for name in ("libcudart.so.12", "libcudart.so.13", "libcudart.so"):
             try:
@@ -59,6 +68,9 @@ class Library:
                 break
             except OSError:
                 continue
+        get_device = 0 if self._get_device is None else C.cast(self._get_device, C.c_void_p).value
+        self.norm, self.scaled, self.w4 = ((self._address[name], get_device) for name in
+                                           ("imd_norm_quantize", "imd_scaled_linear", "imd_linear_w4"))
 
     def device_error(self):
         """imd_linear_device_error: the sticky error word, read and cleared (synchronises)."""
@@ -99,12 +111,19 @@ def load_library(path=None):
 _torch_types = {}   # dtype object of PyTorch -> type (None: not one of ours)
 
 
+def _learn(dtype, kind):
+    from . import _fastcall
+    _fastcall.learn(dtype, kind)
+
+
 def _view(x, what, stream, device):
     """(pointer, shape, element strides or None, type, readonly) of a CUDA array."""
     dtype = getattr(x, "dtype", None)
     if dtype is not None and hasattr(x, "data_ptr"):   # a PyTorch tensor: no capsule is made
         if dtype not in _torch_types:
             _torch_types[dtype] = _TORCH_TYPES.get(str(dtype))
+            if _torch_types[dtype] is not None:
+                _learn(dtype, _torch_types[dtype])
         on = x.get_device()
         if on < 0:
             raise TypeError(f"{what} is not in CUDA memory")
@@ -127,15 +146,6 @@ def _view(x, what, stream, device):
 
 def _matrix(x, what, types, stream, device, out=False):
     """(pointer, rows, columns, row stride, type) of a matrix whose rows have unit stride."""
-    # the usual case in the fewest steps: a call costs as much on the host as on the GPU at one row
-    kind = _torch_types.get(getattr(x, "dtype", None))
-    if kind in types and x.get_device() == device:
-        shape = x.shape
-        if len(shape) == 2:
-            rows, cols = shape
-            strides = x.stride()
-            if strides[1] == 1:
-                return x.data_ptr(), rows, cols, strides[0], kind
     ptr, shape, strides, kind, readonly = _view(x, what, stream, device)
     if kind not in types:
         raise TypeError(f"{what}: dtype must be {' or '.join(_NAMES[t] for t in types)}")
@@ -153,9 +163,6 @@ def _matrix(x, what, types, stream, device, out=False):
 
 def _vector(x, what, n, types, stream, device, out=False):
     """(pointer, type) of a contiguous vector of n elements."""
-    kind = _torch_types.get(getattr(x, "dtype", None))
-    if kind in types and x.get_device() == device and x.shape == (n,) and x.stride(0) == 1:
-        return x.data_ptr(), kind
     ptr, shape, strides, kind, readonly = _view(x, what, stream, device)
     if kind not in types:
         raise TypeError(f"{what}: dtype must be {' or '.join(_NAMES[t] for t in types)}")
@@ -184,28 +191,31 @@ def norm_quantize(x, weight, q, scale, *, eps=1e-6, residual=None, residual_out=
     a row with a NaN or an infinity gives scale NaN. Returns (q, scale)."""
     lib = load_library(lib)
     s = 0 if stream is None else _arrays.stream_handle(stream)
+    st = lib.fast.norm_quantize(*lib.norm, s, x, weight, q, scale, eps, residual, residual_out)
+    if st is None:
+        st = _norm_quantize(lib, s, x, weight, q, scale, eps, residual, residual_out)
+    if st:
+        raise _error(st, "imd_norm_quantize")
+    return q, scale
+
+
+def _norm_quantize(lib, s, x, weight, q, scale, eps, residual, residual_out):
     dev = lib.current_device()
     px, rows, dim, sx, tx = _matrix(x, "x", (F32, BF16, F16), s, dev)
     pw, tw = _vector(weight, "weight", dim, (tx, F32) if tx != F32 else (F32,), s, dev)
     pq, qr, qc, sq, tq = _matrix(q, "q", (I8, E4M3), s, dev, True)
-    if qr != rows or qc != dim:
-        _same("q", (qr, qc), (rows, dim))
+    _same("q", (qr, qc), (rows, dim))
     ps, _ = _vector(scale, "scale", rows, (F32,), s, dev, True)
     pr = sr = ph = sh = 0
     if residual is not None:
         pr, r, c, sr, _ = _matrix(residual, "residual", (tx,), s, dev)
-        if r != rows or c != dim:
-            _same("residual", (r, c), (rows, dim))
+        _same("residual", (r, c), (rows, dim))
     if residual_out is not None:
         if residual is None:
             raise ValueError("residual_out is given without a residual")
         ph, r, c, sh, _ = _matrix(residual_out, "residual_out", (tx,), s, dev, True)
-        if r != rows or c != dim:
-            _same("residual_out", (r, c), (rows, dim))
-    st = lib.lib.imd_norm_quantize(rows, dim, tx, px, sx, pr, sr, tw, pw, eps, ph, sh, tq, pq, sq, ps, s)
-    if st:
-        raise _error(st, "imd_norm_quantize")
-    return q, scale
+        _same("residual_out", (r, c), (rows, dim))
+    return lib.lib.imd_norm_quantize(rows, dim, tx, px, sx, pr, sr, tw, pw, eps, ph, sh, tq, pq, sq, ps, s)
 
 
 def scaled_linear(x, w, out, x_scale, w_scale, *, stream=None, lib=None):
@@ -215,6 +225,15 @@ def scaled_linear(x, w, out, x_scale, w_scale, *, stream=None, lib=None):
     x_scale: [rows], w_scale: [n] float32; out: [rows, n] float32, bfloat16 or float16. Returns out."""
     lib = load_library(lib)
     s = 0 if stream is None else _arrays.stream_handle(stream)
+    st = lib.fast.scaled_linear(*lib.scaled, s, x, w, out, x_scale, w_scale)
+    if st is None:
+        st = _scaled_linear(lib, s, x, w, out, x_scale, w_scale)
+    if st:
+        raise _error(st, "imd_scaled_linear")
+    return out
+
+
+def _scaled_linear(lib, s, x, w, out, x_scale, w_scale):
     dev = lib.current_device()
     px, rows, k, sx, tx = _matrix(x, "x", (I8, E4M3), s, dev)
     pw, n, wk, sw, _ = _matrix(w, "w", (tx,), s, dev)
@@ -223,10 +242,7 @@ def scaled_linear(x, w, out, x_scale, w_scale, *, stream=None, lib=None):
     _same("out", (r, c), (rows, n))
     pxs, _ = _vector(x_scale, "x_scale", rows, (F32,), s, dev)
     pws, _ = _vector(w_scale, "w_scale", n, (F32,), s, dev)
-    st = lib.lib.imd_scaled_linear(rows, n, k, tx, px, sx, pw, sw, pxs, pws, to, po, so, s)
-    if st:
-        raise _error(st, "imd_scaled_linear")
-    return out
+    return lib.lib.imd_scaled_linear(rows, n, k, tx, px, sx, pw, sw, pxs, pws, to, po, so, s)
 
 
 def linear_w4(x, w, out, w_scale, *, zeros=None, group=128, stream=None, lib=None):
@@ -238,6 +254,15 @@ def linear_w4(x, w, out, w_scale, *, zeros=None, group=128, stream=None, lib=Non
     Returns out."""
     lib = load_library(lib)
     s = 0 if stream is None else _arrays.stream_handle(stream)
+    st = lib.fast.linear_w4(*lib.w4, s, x, w, out, w_scale, zeros, group)
+    if st is None:
+        st = _linear_w4(lib, s, x, w, out, w_scale, zeros, group)
+    if st:
+        raise _error(st, "imd_linear_w4")
+    return out
+
+
+def _linear_w4(lib, s, x, w, out, w_scale, zeros, group):
     dev = lib.current_device()
     if group not in (32, 64, 128):
         raise ValueError("group must be 32, 64 or 128")
@@ -253,7 +278,4 @@ def linear_w4(x, w, out, w_scale, *, zeros=None, group=128, stream=None, lib=Non
         _same("zeros", (r, c), (n, groups))
     po, r, c, so, to = _matrix(out, "out", (F32, tx), s, dev, True)
     _same("out", (r, c), (rows, n))
-    st = lib.lib.imd_linear_w4(rows, n, k, group, tx, px, sx, pw, sw, ts, pws, ss, pz, sz, to, po, so, s)
-    if st:
-        raise _error(st, "imd_linear_w4")
-    return out
+    return lib.lib.imd_linear_w4(rows, n, k, group, tx, px, sx, pw, sw, ts, pws, ss, pz, sz, to, po, so, s)
