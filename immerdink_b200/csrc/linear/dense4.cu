@@ -201,6 +201,7 @@ k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUte
     __syncwarp();
   } else if (wg == 1) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsUnpack));
+    const Nibbles<X> nibbles;
     const int r = threadIdx.x & 127;
     const int64_t row = min(n0 + r, p.a.n - 1);
     const uint8_t* w = static_cast<const uint8_t*>(p.a.w) + row * p.a.w_stride;
@@ -266,7 +267,7 @@ k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUte
 #pragma unroll
       for (int i = 0; i < 8; ++i) {  // 16 bytes = 8 weights; the swizzle exchanges the pieces of a row by its number mod 8
         uint32_t o[4];
-        nibble_pairs<X>(q[i], zero[i >> 2], o);
+        nibbles.pairs(q[i], zero[i >> 2], o);
         asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst + ((i ^ (r & 7)) << 4)),
                      "r"(__byte_perm(o[0], o[1], 0x5410)), "r"(__byte_perm(o[2], o[3], 0x5410)),
                      "r"(__byte_perm(o[0], o[1], 0x7632)), "r"(__byte_perm(o[2], o[3], 0x7632))

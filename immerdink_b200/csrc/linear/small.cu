@@ -59,6 +59,7 @@ __global__ void __launch_bounds__(32 * kWarps) k_small_w4(const __grid_constant_
   const int64_t w_end = (p.k + 1) / 2;
   const Span span_w = span_of(p.w, p.n, p.w_stride, w_end), span_x = span_of(p.x, p.rows, 2 * p.x_stride, 2 * p.k);
   const int64_t groups = (p.k + GROUP - 1) / GROUP;
+  const Nibbles<X> nibbles;
   float acc[NT][4] = {};
   for (int64_t g = warp; g < groups; g += kWarps) {
     const int64_t k0 = g * GROUP + (lane & 3) * (GROUP / 4);
@@ -87,7 +88,7 @@ __global__ void __launch_bounds__(32 * kWarps) k_small_w4(const __grid_constant_
     for (int i = 0; i < kWords; ++i) {
       uint32_t a[2][4];  // [row][pair]: pairs (0, 4), (1, 5), (2, 6), (3, 7) of the word
 #pragma unroll
-      for (int h = 0; h < 2; ++h) nibble_pairs<X>(q[h][i], zero[h], a[h]);
+      for (int h = 0; h < 2; ++h) nibbles.pairs(q[h][i], zero[h], a[h]);
       const uint32_t a01[4] = {a[0][0], a[1][0], a[0][1], a[1][1]}, a23[4] = {a[0][2], a[1][2], a[0][3], a[1][3]};
 #pragma unroll
       for (int j = 0; j < NT; ++j) {

@@ -160,7 +160,7 @@ struct Source {
 
 // One step of a tile: `row` is this lane's first row in the slot, `half` the step's 64 bytes of it.
 template <typename C>
-__device__ __forceinline__ void multiply(const Ready<C>& q, uint32_t row, int half, int lane, float (&acc)[C::MT][C::NT][4]) {
+__device__ __forceinline__ void multiply(const Ready<C>& q, const Nibbles<typename C::X>& nibbles, uint32_t row, int half, int lane, float (&acc)[C::MT][C::NT][4]) {
   using X = typename C::X;
 #pragma unroll
   for (int g = 0; g < C::kPerStep; ++g) {
@@ -181,7 +181,7 @@ __device__ __forceinline__ void multiply(const Ready<C>& q, uint32_t row, int ha
       for (int i = 0; i < C::kWords; ++i) {
         uint32_t a[2][4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) nibble_pairs<X>(w[h][i], z[h], a[h]);
+        for (int h = 0; h < 2; ++h) nibbles.pairs(w[h][i], z[h], a[h]);
         const uint32_t a01[4] = {a[0][0], a[1][0], a[0][1], a[1][1]}, a23[4] = {a[0][2], a[1][2], a[0][3], a[1][3]};
 #pragma unroll
         for (int j = 0; j < C::NT; ++j) {
@@ -218,56 +218,56 @@ k_stream(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ Para
   __syncthreads();
 
   // the warp's pieces: warp, warp + 8, ... of each tile of the CTA
-  const int mine = (p.pieces - warp + kWarps - 1) / kWarps;
+  const int mine = (p.pieces - warp + kWarps - 1) / kWarps, tiles = static_cast<int>(p.tiles);
   const uint64_t policy = l2_policy(2);  // weights pass through once
-  int64_t load_tile = blockIdx.x;
-  int load_step = 0;
+  int load_row = mine > 0 ? static_cast<int>(blockIdx.x) * kRows : tiles * kRows, load_step = 0;
   auto load = [&](int slot) {  // the next piece of the walk into `slot`, by one lane
-    if (mine <= 0 || load_tile >= p.tiles) return;
+    if (load_row >= tiles * kRows) return;
     if (lane == 0) {
       mbar_expect_tx(bar(slot), kSlotBytes);
-      tma_load_3d(ring + slot * kSlotBytes, &map_w, bar(slot), (load_step * kWarps + warp) * (kPieceK / 2),
-                  static_cast<int>(load_tile * kRows), 0, policy);
+      tma_load_3d(ring + slot * kSlotBytes, &map_w, bar(slot), (load_step * kWarps + warp) * (kPieceK / 2), load_row, 0, policy);
     }
-    if (++load_step == mine) load_step = 0, load_tile += gridDim.x;
+    if (++load_step == mine) load_step = 0, load_row += gridDim.x * kRows;
   };
   for (int s = 0; s < p.slots; ++s) load(s);
 
   Source<C> source(p.a, lane);
+  const Nibbles<typename C::X> nibbles;
   Raw<C> raw;
-  const int steps = 2 * mine;  // of 128 k
-  auto k_of = [&](int step) { return ((step >> 1) * kWarps + warp) * kPieceK + (step & 1) * 128; };
+  const int k_first = warp * kPieceK;
   if (mine > 0 && blockIdx.x < p.tiles) {
     source.set_tile(p.a, static_cast<int64_t>(blockIdx.x) * kRows, lane);
-    source.fetch(k_of(0), lane, raw);
+    source.fetch(k_first, lane, raw);
   }
   int slot = 0, turn = 0;
   uint32_t phase = 0;
-  for (int64_t tile = blockIdx.x; tile < p.tiles; tile += gridDim.x) {
-    const int64_t n0 = tile * kRows;
+  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    const int64_t n0 = static_cast<int64_t>(tile) * kRows;
     float acc[MT][NT][4] = {};
+    int k0 = k_first;
 #pragma unroll 1
-    for (int step = 0; step < steps; ++step) {
+    for (int left = mine; left > 0; --left) {
+      const uint32_t row = ring + slot * kSlotBytes + (lane >> 2) * 128;
       Ready<C> ready;
       source.settle(raw, ready);
-      if (step + 1 < steps) {
-        source.fetch(k_of(step + 1), lane, raw);
-      } else if (tile + gridDim.x < p.tiles) {
-        source.set_tile(p.a, (tile + gridDim.x) * kRows, lane);
-        source.fetch(k_of(0), lane, raw);
+      source.fetch(k0 + 128, lane, raw);
+      mbar_wait(bar(slot), phase, abort);  // after a wait that gave up the values are of no use, but every barrier is passed
+      __syncwarp();
+      multiply<C>(ready, nibbles, row, 0, lane, acc);
+      source.settle(raw, ready);
+      k0 += kWarps * kPieceK;
+      if (left > 1) {
+        source.fetch(k0, lane, raw);
+      } else if (tile + static_cast<int>(gridDim.x) < tiles) {
+        source.set_tile(p.a, n0 + static_cast<int64_t>(gridDim.x) * kRows, lane);
+        source.fetch(k_first, lane, raw);
       }
-      if ((step & 1) == 0) {
-        mbar_wait(bar(slot), phase, abort);  // after a wait that gave up the values are of no use, but every barrier is passed
-        __syncwarp();
-      }
-      multiply<C>(ready, ring + slot * kSlotBytes + (lane >> 2) * 128, step & 1, lane, acc);
-      if ((step & 1) != 0) {
-        __syncwarp();
-        load(slot);
-        if (++slot == p.slots) {
-          slot = 0;
-          phase ^= 1u;
-        }
+      multiply<C>(ready, nibbles, row, 1, lane, acc);
+      __syncwarp();
+      load(slot);
+      if (++slot == p.slots) {
+        slot = 0;
+        phase ^= 1u;
       }
     }
 #pragma unroll

@@ -96,16 +96,24 @@ __device__ __forceinline__ uint32_t sub_pair(uint32_t a, uint32_t b, __nv_bfloat
   __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
   return *reinterpret_cast<uint32_t*>(&r);
 }
-// The pairs (w_i - z, w_i+4 - z), i = 0..3, of the eight nibbles of a word; zero = magic | z | z << 16.
-// (word & mask) | magic is one lop3 when written as one; from C++ the compiler makes two of it.
+// The two constants of the unpacking, in registers: the compiler would materialise them again at each use.
 template <typename X>
-__device__ __forceinline__ void nibble_pairs(uint32_t word, uint32_t zero, uint32_t* pair) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t v;
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(v) : "r"(word >> (4 * i)), "r"(0x000F000Fu), "r"(nibble_magic<X>()));
-    pair[i] = sub_pair(v, zero, X());
+struct Nibbles {
+  uint32_t mask, magic;
+  __device__ __forceinline__ Nibbles() {
+    asm volatile("mov.u32 %0, 0x000F000F;" : "=r"(mask));
+    asm volatile("mov.u32 %0, %1;" : "=r"(magic) : "n"(nibble_magic<X>()));
   }
-}
+  // The pairs (w_i - z, w_i+4 - z), i = 0..3, of the eight nibbles of a word; zero = magic | z | z << 16.
+  // (word & mask) | magic is one lop3 when written as one; from C++ the compiler makes two of it.
+  __device__ __forceinline__ void pairs(uint32_t word, uint32_t zero, uint32_t* pair) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t v;
+      asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(v) : "r"(word >> (4 * i)), "r"(mask), "r"(magic));
+      pair[i] = sub_pair(v, zero, X());
+    }
+  }
+};
 
 }  // namespace imd
