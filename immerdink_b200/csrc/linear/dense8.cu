@@ -291,6 +291,7 @@ k_dense8_pair(const __grid_constant__ CUtensorMap map_x, const __grid_constant__
 }
 
 // ---- up to 256 rows: weights on the M side ---------------------------------------------------------------
+constexpr int kSwapThreads = 320;  // warp 0 TMA, warp 1 MMA, warps 2-9 epilogue
 constexpr int kSwapMaxStages = 12;
 constexpr int kFoldCols = 64;  // columns folded through shared memory at a time: 128 x 64 x 4 bytes
 
@@ -300,8 +301,77 @@ __device__ __forceinline__ uint32_t load_cluster(uint32_t addr) {
   return v;
 }
 
+// Accumulators to outputs. Warps 2-9: two per quarter of the tensor memory's lanes (= rows of w), which take the
+// columns (= rows of x) by turns of 32. A warp's stores are 32 neighbours of one output row.
+template <bool I8, typename T>
+__device__ __forceinline__ void swap_epilogue(const Params& p, uint32_t tmem_base, uint32_t tiles, const float* x_scale, int n0,
+                                              int part, int parts) {
+  const int warp = threadIdx.x >> 5, quarter = warp & 3, turn = warp < 6 ? 0 : 1;
+  const int row = quarter * 32 + static_cast<int>(threadIdx.x & 31);
+  const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+  const bool inside = n0 + row < p.n;
+  const float ws = inside ? p.w_scale[n0 + row] : 0.0f;
+  T* out = static_cast<T*>(p.out) + n0 + row;
+  if (parts == 1) {
+    if (warp >= 2) {
+#pragma unroll 1
+      for (int c = 32 * turn; c < p.cols; c += 64) {
+        uint32_t v[32];
+        tmem_load_32(taddr + c, v);
+        if (inside) {
+          T* o = out + c * p.out_stride;
+#pragma unroll
+          for (int j = 0; j < 32; ++j, o += p.out_stride)
+            if (c + j < p.rows) *o = from_float<T>(acc_value<I8>(v[j]) * x_scale[c + j] * ws);
+        }
+        __syncwarp();
+      }
+    }
+    return;
+  }
+  for (int c0 = 0; c0 < p.cols; c0 += kFoldCols) {
+    const int width = min(kFoldCols, p.cols - c0);
+    if (warp >= 2) {
+      for (int c = 32 * turn; c < width; c += 64) {
+        uint32_t v[32];
+        tmem_load_32(taddr + c0 + c, v);
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (c + j < width)
+            asm volatile("st.shared.u32 [%0], %1;" ::"r"(tiles + ((c + j) * kTileM + row) * 4), "r"(v[j]) : "memory");
+      }
+    }
+    __syncwarp();
+    cluster_sync_all();
+    // part r adds columns r, r + parts, ..., eight at a time so that the remote loads overlap
+    if (warp >= 2 && inside) {
+      const int last = min(width, p.rows - c0), step = 2 * parts;
+      for (int c = part + parts * turn; c < last; c += 8 * step) {
+        uint32_t v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = 0;  // also 0.0f
+        for (int r = 0; r < parts; ++r) {
+          const uint32_t base = map_to_cta(tiles + row * 4, r);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int cj = c + j * step;
+            const uint32_t u = cj < last ? load_cluster(base + cj * kTileM * 4) : 0u;
+            v[j] = I8 ? v[j] + u : __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(u));
+          }
+        }
+        T* o = out + (c0 + c) * p.out_stride;
+#pragma unroll
+        for (int j = 0; j < 8; ++j, o += step * p.out_stride)
+          if (c + j * step < last) *o = from_float<T>(acc_value<I8>(v[j]) * x_scale[c0 + c + j * step] * ws);
+      }
+    }
+    __syncwarp();
+    cluster_sync_all();  // the peers have read this CTA's columns
+  }
+}
+
 template <bool I8>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kSwapThreads)
 k_dense8_swap(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
               const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem_raw[];
@@ -321,6 +391,8 @@ k_dense8_swap(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
   const int kb0 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * part / parts);
   const int kb1 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * (part + 1) / parts);
   const int n0 = blockIdx.x * kTileM;
+  __shared__ float x_scale[256];
+  for (int i = threadIdx.x; i < p.cols; i += kSwapThreads) x_scale[i] = i < p.rows ? p.x_scale[i] : 0.0f;
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) {
       mbar_init(full(s), 1);
@@ -396,68 +468,9 @@ k_dense8_swap(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
   tc_fence_after();
   __syncthreads();
 
-  const int quarter = warp & 3;
-  const int row = quarter * 32 + lane;                       // of the tile: a row of w
-  const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
-  const float ws = n0 + row < p.n ? p.w_scale[n0 + row] : 0.0f;
-  if (parts == 1) {
-    if (warp >= 2) {
-#pragma unroll 1
-      for (int c = 0; c < p.cols; c += 32) {
-        uint32_t v[32];
-        tmem_load_32(taddr + c, v);
-        if (n0 + row < p.n) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (c + j < p.rows)
-              store_out(p.out, p.out_type, (c + j) * p.out_stride + n0 + row, acc_value<I8>(v[j]) * __ldg(p.x_scale + c + j) * ws);
-        }
-        __syncwarp();
-      }
-    }
-  } else {
-    for (int c0 = 0; c0 < p.cols; c0 += kFoldCols) {
-      const int width = min(kFoldCols, p.cols - c0);
-      if (warp >= 2) {
-        for (int c = 0; c < width; c += 32) {
-          uint32_t v[32];
-          tmem_load_32(taddr + c0 + c, v);
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (c + j < width)
-              asm volatile("st.shared.u32 [%0], %1;" ::"r"(tiles + ((c + j) * kTileM + row) * 4), "r"(v[j]) : "memory");
-        }
-      }
-      __syncwarp();
-      cluster_sync_all();
-      // part r adds columns r, r + parts, ..., eight at a time so that the remote loads overlap
-      if (warp >= 2 && n0 + row < p.n) {
-        const int last = min(width, p.rows - c0);
-        for (int c = part; c < last; c += 8 * parts) {
-          uint32_t v[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = 0;  // also 0.0f
-          for (int r = 0; r < parts; ++r) {
-            const uint32_t base = map_to_cta(tiles + row * 4, r);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const int cj = c + j * parts;
-              const uint32_t u = cj < last ? load_cluster(base + cj * kTileM * 4) : 0u;
-              v[j] = I8 ? v[j] + u : __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(u));
-            }
-          }
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int cj = c0 + c + j * parts;
-            if (cj < c0 + last)
-              store_out(p.out, p.out_type, cj * p.out_stride + n0 + row, acc_value<I8>(v[j]) * p.x_scale[cj] * ws);
-          }
-        }
-      }
-      __syncwarp();
-      cluster_sync_all();  // the peers have read this CTA's columns
-    }
-  }
+  if (p.out_type == IMD_TYPE_F32) swap_epilogue<I8, float>(p, tmem_base, tiles, x_scale, n0, part, parts);
+  else if (p.out_type == IMD_TYPE_F16) swap_epilogue<I8, __half>(p, tmem_base, tiles, x_scale, n0, part, parts);
+  else swap_epilogue<I8, __nv_bfloat16>(p, tmem_base, tiles, x_scale, n0, part, parts);
   tc_fence_before();
   __syncthreads();
   if (threadIdx.x == 0 && *abort) atomicOr(p.error_word, 1u);
@@ -507,7 +520,7 @@ bool launch_swap(const LinearArgs& a, const DeviceInfo& dev, Params p, cudaStrea
   if (p.stages > kSwapMaxStages) p.stages = kSwapMaxStages;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned int>(tiles), static_cast<unsigned int>(parts));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(kSwapThreads);
   cfg.dynamicSmemBytes = static_cast<size_t>(p.stages) * stage_bytes + 1024 + kCtrlBytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
