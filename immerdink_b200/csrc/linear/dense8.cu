@@ -293,7 +293,6 @@ k_dense8_pair(const __grid_constant__ CUtensorMap map_x, const __grid_constant__
 // ---- up to 256 rows: weights on the M side ---------------------------------------------------------------
 constexpr int kSwapThreads = 320;  // warp 0 TMA, warp 1 MMA, warps 2-9 epilogue
 constexpr int kSwapMaxStages = 12;
-constexpr int kFoldCols = 64;  // columns folded through shared memory at a time: 128 x 64 x 4 bytes
 
 __device__ __forceinline__ uint32_t load_cluster(uint32_t addr) {
   uint32_t v;
@@ -329,45 +328,43 @@ __device__ __forceinline__ void swap_epilogue(const Params& p, uint32_t tmem_bas
     }
     return;
   }
-  for (int c0 = 0; c0 < p.cols; c0 += kFoldCols) {
-    const int width = min(kFoldCols, p.cols - c0);
-    if (warp >= 2) {
-      for (int c = 32 * turn; c < width; c += 64) {
-        uint32_t v[32];
-        tmem_load_32(taddr + c0 + c, v);
+  // every column's partial sums fit the ring's memory: 512 bytes a column, and a stage has 128 of them and 16 KB
+  if (warp >= 2) {
+    for (int c = 32 * turn; c < p.cols; c += 64) {
+      uint32_t v[32];
+      tmem_load_32(taddr + c, v);
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (c + j < width)
-            asm volatile("st.shared.u32 [%0], %1;" ::"r"(tiles + ((c + j) * kTileM + row) * 4), "r"(v[j]) : "memory");
-      }
+      for (int j = 0; j < 32; ++j)
+        if (c + j < p.cols)
+          asm volatile("st.shared.u32 [%0], %1;" ::"r"(tiles + ((c + j) * kTileM + row) * 4), "r"(v[j]) : "memory");
     }
-    __syncwarp();
-    cluster_sync_all();
-    // part r adds columns r, r + parts, ..., eight at a time so that the remote loads overlap
-    if (warp >= 2 && inside) {
-      const int last = min(width, p.rows - c0), step = 2 * parts;
-      for (int c = part + parts * turn; c < last; c += 8 * step) {
-        uint32_t v[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = 0;  // also 0.0f
-        for (int r = 0; r < parts; ++r) {
-          const uint32_t base = map_to_cta(tiles + row * 4, r);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int cj = c + j * step;
-            const uint32_t u = cj < last ? load_cluster(base + cj * kTileM * 4) : 0u;
-            v[j] = I8 ? v[j] + u : __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(u));
-          }
-        }
-        T* o = out + (c0 + c) * p.out_stride;
-#pragma unroll
-        for (int j = 0; j < 8; ++j, o += step * p.out_stride)
-          if (c + j * step < last) *o = from_float<T>(acc_value<I8>(v[j]) * x_scale[c0 + c + j * step] * ws);
-      }
-    }
-    __syncwarp();
-    cluster_sync_all();  // the peers have read this CTA's columns
   }
+  __syncwarp();
+  cluster_sync_all();
+  // part r adds columns r, r + parts, ..., eight at a time so that the remote loads overlap
+  if (warp >= 2 && inside) {
+    const int step = 2 * parts;
+    for (int c = part + parts * turn; c < p.rows; c += 8 * step) {
+      uint32_t v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = 0;  // also 0.0f
+      for (int r = 0; r < parts; ++r) {
+        const uint32_t base = map_to_cta(tiles + row * 4, r);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int cj = c + j * step;
+          const uint32_t u = cj < p.rows ? load_cluster(base + cj * kTileM * 4) : 0u;
+          v[j] = I8 ? v[j] + u : __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(u));
+        }
+      }
+      T* o = out + c * p.out_stride;
+#pragma unroll
+      for (int j = 0; j < 8; ++j, o += step * p.out_stride)
+        if (c + j * step < p.rows) *o = from_float<T>(acc_value<I8>(v[j]) * x_scale[c + j * step] * ws);
+    }
+  }
+  __syncwarp();
+  cluster_sync_all();  // the peers have read this CTA's columns
 }
 
 template <bool I8>
@@ -518,6 +515,7 @@ bool launch_swap(const LinearArgs& a, const DeviceInfo& dev, Params p, cudaStrea
   const int stage_bytes = kBytesM + p.cols * kTileK;
   p.stages = ((two ? kSwapSmemHalf : kSwapSmem) - 1024 - kCtrlBytes) / stage_bytes;
   if (p.stages > kSwapMaxStages) p.stages = kSwapMaxStages;
+  if (static_cast<int64_t>(p.stages) * stage_bytes < static_cast<int64_t>(p.cols) * kTileM * 4) return false;  // (the fold)
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned int>(tiles), static_cast<unsigned int>(parts));
   cfg.blockDim = dim3(kSwapThreads);
