@@ -12,6 +12,7 @@
 // Warpgroups (512 threads, 128 registers each at launch, shared out again by setmaxnreg):
 //   0     warp 0 brings x by TMA (64 k = 128 bytes of a row, 128-byte swizzle), warp 1 issues the MMAs, warp 2
 //         brings the packed weights by TMA, 256 k (128 bytes of a row) at a time into two slots of their own
+//         (rows that TMA cannot bring: x by warpgroups 2 and 3, each row's weights by the thread that unpacks it)
 //   1     thread r turns row r of the weights' next 64 k into 16-bit floats in the swizzled layout
 //   2, 3  halves of the rows of x: out += scale * accumulator, then the stores
 // Bound by shared memory traffic for many rows (the operand tiles are written and read at about the port's rate),
@@ -64,7 +65,7 @@ __device__ __forceinline__ uint32_t load_cluster(uint32_t addr) {
   return v;
 }
 
-template <typename X, int GROUP>
+template <typename X, int GROUP, bool ANY>
 __global__ void __launch_bounds__(kThreads, 1)
 k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
          const __grid_constant__ Params p) {
@@ -95,7 +96,7 @@ k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUte
   const int64_t n0 = static_cast<int64_t>(blockIdx.x / p.tiles_t) * kTileM;
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) {
-      mbar_init(full(s), 1 + 4);  // the TMA producer's arrival, and the four unpacking warps
+      mbar_init(full(s), (ANY ? 8 : 1) + 4);  // who brings x, and the four unpacking warps
       mbar_init(empty(s), 1);
     }
     for (int a = 0; a < 2; ++a) {
@@ -121,7 +122,7 @@ k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUte
 
   if (wg == 0) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
-    if (warp == 0 && lane == 0) {
+    if (!ANY && warp == 0 && lane == 0) {
       int stage = 0;
       uint32_t phase = 0, issued = 0;
       bool okay = true;
@@ -308,6 +309,31 @@ k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUte
     float scale[4], next[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) next[i] = scale_of(g0 + i);
+    // ANY: rows of x that TMA cannot bring. These warps bring them, as far ahead as the ring allows: a stage is free
+    // once the group that used it is complete.
+    const int blocks = (u1 - u0) * kBlocks;
+    const Span span = span_of(p.a.x, p.a.rows, 2 * p.a.x_stride, 2 * p.a.k);
+    int brought = 0, stage = 0;
+    uint32_t phase = 0;
+    auto bring = [&](int limit) {
+#pragma unroll 1
+      for (; brought < min(limit, blocks); ++brought) {
+        if (!mbar_wait(empty(stage), phase ^ 1u, abort)) break;
+        const int64_t at = static_cast<int64_t>(u0 * kBlocks + brought) * 2 * kBlockK;
+#pragma unroll 1
+        for (int r = warp - 8; r < p.cols; r += 64)
+          bring_rows<8>(static_cast<const uint8_t*>(p.a.x), 2 * p.a.x_stride, p.a.rows, t0, r, 8, p.cols, at, 2 * p.a.k, span,
+                        tiles + stage * stage_bytes + kBytesM);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full(stage));
+        if (++stage == p.stages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    };
+    if (ANY) bring(p.stages);
 #pragma unroll 1
     for (int g = g0; g < g1; ++g) {
       const int i = (g - g0) & 3;
@@ -335,6 +361,7 @@ k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUte
       if (lane == 0) mbar_arrive(tempty(acc));
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1u;
+      if (ANY) bring((g + 1 - g0) * GROUP / kBlockK + p.stages);
     }
     __syncwarp();
     if (parts == 1) {
@@ -392,8 +419,9 @@ k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUte
 
 using Kernel = void (*)(const CUtensorMap, const CUtensorMap, const Params);
 template <typename X>
-Kernel kernel_of(int group) {
-  return group == 128 ? k_dense4<X, 128> : group == 64 ? k_dense4<X, 64> : k_dense4<X, 32>;
+Kernel kernel_of(int group, bool any) {
+  if (any) return group == 128 ? k_dense4<X, 128, true> : group == 64 ? k_dense4<X, 64, true> : k_dense4<X, 32, true>;
+  return group == 128 ? k_dense4<X, 128, false> : group == 64 ? k_dense4<X, 64, false> : k_dense4<X, 32, false>;
 }
 
 }  // namespace
@@ -401,7 +429,8 @@ Kernel kernel_of(int group) {
 // The shares above are drawn from the registers of the launch, so a kernel compiled for fewer is refused.
 bool dense4_setup() {
   for (int group : {32, 64, 128})
-    for (Kernel k : {kernel_of<__half>(group), kernel_of<__nv_bfloat16>(group)}) {
+    for (Kernel k : {kernel_of<__half>(group, false), kernel_of<__nv_bfloat16>(group, false), kernel_of<__half>(group, true),
+                     kernel_of<__nv_bfloat16>(group, true)}) {
       cudaFuncAttributes attr;
       const void* f = reinterpret_cast<const void*>(k);
       if (cudaFuncGetAttributes(&attr, f) != cudaSuccess || attr.numRegs < kRegsLaunch ||
@@ -411,8 +440,12 @@ bool dense4_setup() {
   return true;
 }
 
+// Rows of any alignment with little work are quicker in the small kernel: 1802 x 83 x 150 9 against 27 us; 100 x 4000 x
+// 1001 26 against 24 us, 1000 x 4000 x 1001 218 against 109 us.
+constexpr int64_t kLeastWork = INT64_C(1) << 28;
 bool dense4_takes(const LinearArgs& a) {
-  return a.kind == WeightKind::kU4 && a.k > 0 && a.rows > 16 && rows_for_tma(a.x, a.rows, 2 * a.x_stride, 2 * a.k);
+  return a.kind == WeightKind::kU4 && a.k > 0 && a.rows > 16 &&
+         (rows_for_tma(a.x, a.rows, 2 * a.x_stride, 2 * a.k) || a.rows * a.n * a.k >= kLeastWork);
 }
 
 imd_status_t dense4_launch(const LinearArgs& a, cudaStream_t stream) {
@@ -433,8 +466,9 @@ imd_status_t dense4_launch(const LinearArgs& a, cudaStream_t stream) {
   if (p.stages > kMaxStages) p.stages = kMaxStages;
 
   // the swizzle goes by bytes, so x is described as bytes too
-  CUtensorMap map_x, map_w{};
-  if (!encode_rows_128(*dev, &map_x, a.x, 2 * a.k, a.rows, 2 * a.x_stride, p.cols) ||
+  const bool any = !rows_for_tma(a.x, a.rows, 2 * a.x_stride, 2 * a.k);
+  CUtensorMap map_x{}, map_w{};
+  if ((!any && !encode_rows_128(*dev, &map_x, a.x, 2 * a.k, a.rows, 2 * a.x_stride, p.cols)) ||
       (p.wide && !encode_rows_128(*dev, &map_w, a.w, (a.k + 1) / 2, a.n, a.w_stride, kTileM)))
     return IMD_STATUS_CUDA_ERROR;
 
@@ -452,7 +486,7 @@ imd_status_t dense4_launch(const LinearArgs& a, cudaStream_t stream) {
   attr[0].val.clusterDim = {1, static_cast<unsigned int>(parts), 1};
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const Kernel k = a.x_type == IMD_TYPE_F16 ? kernel_of<__half>(a.group) : kernel_of<__nv_bfloat16>(a.group);
+  const Kernel k = a.x_type == IMD_TYPE_F16 ? kernel_of<__half>(a.group, any) : kernel_of<__nv_bfloat16>(a.group, any);
   const bool ok = cudaLaunchKernelEx(&cfg, k, map_x, map_w, p) == cudaSuccess;
   return cudaGetLastError() == cudaSuccess && ok ? IMD_STATUS_SUCCESS : IMD_STATUS_CUDA_ERROR;
 }

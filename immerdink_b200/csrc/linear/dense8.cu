@@ -41,6 +41,8 @@ struct Params {
   int64_t out_stride;
   int32_t out_type, out_wide;           // out_wide: 16-byte stores are aligned
   unsigned int* error_word;
+  const uint8_t *x, *w;                 // rows of any alignment: where they are
+  int64_t x_stride, w_stride, k;
 };
 
 // Instruction descriptor: D s32 (2) with A = B = s8 (1), or D f32 (1) with A = B = e4m3 (0); both K-major.
@@ -367,10 +369,20 @@ __device__ __forceinline__ void swap_epilogue(const Params& p, uint32_t tmem_bas
   cluster_sync_all();  // the peers have read this CTA's columns
 }
 
-template <bool I8>
+// ANY: rows that TMA cannot bring. The epilogue's warps, idle until the sums are complete, bring the operands'
+// next 128 bytes per row instead, row by row.
+template <bool I8, bool ANY>
 __global__ void __launch_bounds__(kSwapThreads)
 k_dense8_swap(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
-              const __grid_constant__ Params p) {
+              const __grid_constant__ Params call) {
+  Params p = call;
+  if (ANY) {  // a tile of the rows of x per z
+    const int64_t t0 = static_cast<int64_t>(blockIdx.z) * p.cols;
+    p.x += t0 * p.x_stride;
+    p.x_scale += t0;
+    p.out = static_cast<uint8_t*>(p.out) + t0 * p.out_stride * (p.out_type == IMD_TYPE_F32 ? 4 : 2);
+    p.rows = min(p.cols, static_cast<int32_t>(p.rows - t0));
+  }
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t tiles = (raw + 1023u) & ~1023u;
@@ -392,7 +404,7 @@ k_dense8_swap(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
   for (int i = threadIdx.x; i < p.cols; i += kSwapThreads) x_scale[i] = i < p.rows ? p.x_scale[i] : 0.0f;
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) {
-      mbar_init(full(s), 1);
+      mbar_init(full(s), ANY ? 8 : 1);
       mbar_init(empty(s), 1);
     }
     mbar_init(done, 1);
@@ -410,7 +422,27 @@ k_dense8_swap(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  if (warp == 0) {
+  if (ANY && warp >= 2) {
+    const Span span_w = span_of(p.w, p.n, p.w_stride, p.k), span_x = span_of(p.x, p.rows, p.x_stride, p.k);
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!mbar_wait(empty(stage), phase ^ 1u, abort)) break;
+      const uint32_t dst = tiles + stage * stage_bytes;
+      const int64_t at = static_cast<int64_t>(kb) * kTileK;
+      bring_rows<16>(p.w, p.w_stride, p.n, n0, warp - 2, 8, kTileM, at, p.k, span_w, dst);
+      for (int r = 0; r < p.cols; r += 128)
+        bring_rows<16>(p.x, p.x_stride, p.rows, 0, r + warp - 2, 8, p.cols, at, p.k, span_x, dst + kBytesM);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the tensor core reads through the async proxy
+      __syncwarp();
+      if (lane == 0) mbar_arrive(full(stage));
+      if (++stage == p.stages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+    __syncwarp();
+  } else if (!ANY && warp == 0) {
     if (lane == 0) {
       int stage = 0;
       uint32_t phase = 0, issued = 0;
@@ -499,25 +531,30 @@ bool launch_pair(const LinearArgs& a, const DeviceInfo& dev, Params p, cudaStrea
   return true;
 }
 
-template <bool I8>
+template <bool I8, bool ANY>
 bool launch_swap(const LinearArgs& a, const DeviceInfo& dev, Params p, cudaStream_t stream) {
-  CUtensorMap mx, mw;
-  p.cols = static_cast<int32_t>((a.rows + 15) / 16 * 16);
+  CUtensorMap mx{}, mw{};
+  // rows of x per tile: all of them, or (any alignment) even shares of at most 256
+  const int64_t tiles_t = (a.rows + 255) / 256;
+  p.cols = static_cast<int32_t>(((a.rows + tiles_t - 1) / tiles_t + 15) / 16 * 16);
   p.tmem_cols = 32;
   while (p.tmem_cols < p.cols) p.tmem_cols *= 2;
-  if (!encode_rows_128(dev, &mx, a.x, a.k, a.rows, a.x_stride, p.cols) ||
-      !encode_rows_128(dev, &mw, a.w, a.k, a.n, a.w_stride, kTileM))
+  if (!ANY && (!encode_rows_128(dev, &mx, a.x, a.k, a.rows, a.x_stride, p.cols) ||
+               !encode_rows_128(dev, &mw, a.w, a.k, a.n, a.w_stride, kTileM)))
     return false;
-  const int64_t tiles = (a.n + kTileM - 1) / kTileM;
+  p.x = static_cast<const uint8_t*>(a.x), p.w = static_cast<const uint8_t*>(a.w);
+  p.x_stride = a.x_stride, p.w_stride = a.w_stride, p.k = a.k;
+  const int64_t tiles = (a.n + kTileM - 1) / kTileM, tiles_z = (a.rows + p.cols - 1) / p.cols;
+  if (tiles_z > 65535) return false;
   const bool two = p.cols <= kSwapColsHalf;
   int parts = 1;  // CTAs that share a row tile: enough to occupy the SMs, at least two K blocks each
-  while (parts < 8 && tiles * parts * 2 <= dev.sms * (two ? 2 : 1) && p.k_blocks >= 4 * parts) parts *= 2;
+  while (parts < 8 && tiles * tiles_z * parts * 2 <= dev.sms * (two ? 2 : 1) && p.k_blocks >= 4 * parts) parts *= 2;
   const int stage_bytes = kBytesM + p.cols * kTileK;
   p.stages = ((two ? kSwapSmemHalf : kSwapSmem) - 1024 - kCtrlBytes) / stage_bytes;
   if (p.stages > kSwapMaxStages) p.stages = kSwapMaxStages;
   if (static_cast<int64_t>(p.stages) * stage_bytes < static_cast<int64_t>(p.cols) * kTileM * 4) return false;  // (the fold)
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned int>(tiles), static_cast<unsigned int>(parts));
+  cfg.gridDim = dim3(static_cast<unsigned int>(tiles), static_cast<unsigned int>(parts), static_cast<unsigned int>(tiles_z));
   cfg.blockDim = dim3(kSwapThreads);
   cfg.dynamicSmemBytes = static_cast<size_t>(p.stages) * stage_bytes + 1024 + kCtrlBytes;
   cfg.stream = stream;
@@ -526,7 +563,7 @@ bool launch_swap(const LinearArgs& a, const DeviceInfo& dev, Params p, cudaStrea
   attr[0].val.clusterDim = {1, static_cast<unsigned int>(parts), 1};
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, k_dense8_swap<I8>, mw, mx, p) == cudaSuccess;
+  return cudaLaunchKernelEx(&cfg, k_dense8_swap<I8, ANY>, mw, mx, p) == cudaSuccess;
 }
 
 template <bool I8>
@@ -536,12 +573,15 @@ bool set_attributes() {
   };
   return smem(reinterpret_cast<const void*>(k_dense8_pair<I8, 256>), kPairSmem<256>) &&
          smem(reinterpret_cast<const void*>(k_dense8_pair<I8, 128>), kPairSmem<128>) &&
-         smem(reinterpret_cast<const void*>(k_dense8_swap<I8>), kSwapSmem);
+         smem(reinterpret_cast<const void*>(k_dense8_swap<I8, false>), kSwapSmem) &&
+         smem(reinterpret_cast<const void*>(k_dense8_swap<I8, true>), kSwapSmem);
 }
 
 template <bool I8>
 bool launch(const LinearArgs& a, const DeviceInfo& dev, const Params& p, cudaStream_t stream) {
-  if (a.rows <= 256) return launch_swap<I8>(a, dev, p, stream);
+  if (!rows_for_tma(a.x, a.rows, a.x_stride, a.k) || !rows_for_tma(a.w, a.n, a.w_stride, a.k))
+    return launch_swap<I8, true>(a, dev, p, stream);
+  if (a.rows <= 256) return launch_swap<I8, false>(a, dev, p, stream);
   // whole waves of tiles on the CTA pairs: 128 columns where their last wave is fuller by more than the
   // narrower tile costs
   const int64_t tiles_m = (a.rows + 255) / 256, pairs = dev.sms / 2;
@@ -554,8 +594,12 @@ bool launch(const LinearArgs& a, const DeviceInfo& dev, const Params& p, cudaStr
 
 bool dense8_setup() { return set_attributes<true>() && set_attributes<false>(); }
 
+// The tensor-core kernels take rows of any alignment; with little work those are quicker in the small kernel (int8,
+// 1000 x 300 x 777: 12 against 28 us; 100 x 5000 x 4001: 74 against 54 us, 2000 x 5000 x 4001: 958 against 299 us).
+constexpr int64_t kLeastWork = INT64_C(1) << 30;
 bool dense8_takes(const LinearArgs& a) {
-  return a.kind != WeightKind::kU4 && a.k > 0 && rows_for_tma(a.x, a.rows, a.x_stride, a.k) && rows_for_tma(a.w, a.n, a.w_stride, a.k);
+  if (a.kind == WeightKind::kU4 || a.k == 0) return false;
+  return (a.rows > 16 && a.rows * a.n * a.k >= kLeastWork) || (rows_for_tma(a.x, a.rows, a.x_stride, a.k) && rows_for_tma(a.w, a.n, a.w_stride, a.k));
 }
 
 imd_status_t dense8_launch(const LinearArgs& a, cudaStream_t stream) {

@@ -80,6 +80,58 @@ __device__ __forceinline__ void load_bytes(const uint8_t* row, int64_t at, int64
   }
 }
 
+// 128 bytes of each of ROWS rows of any alignment, by one warp, into shared memory in the layout of a TMA box with the
+// 128-byte swizzle (row r of the box at r * 128, its 16-byte pieces exchanged by r mod 8). A lane loads two
+// neighbouring aligned words of each row and shifts them into place; all loads are issued before the first store.
+// Row i is box row r0 + i * step and starts at base + (row0 + r0 + i * step) * stride; bytes from `end` of a row on and
+// rows from `rows` on are zero. Where a word might lie outside the matrix single bytes are loaded.
+template <int ROWS>
+__device__ __forceinline__ void bring_rows(const uint8_t* base, int64_t stride, int64_t rows, int64_t row0, int r0, int step,
+                                           int box_rows, int64_t at, int64_t end, const Span& span, uint32_t dst) {
+  const int lane = threadIdx.x & 31;
+  const int64_t valid = end - at - 4 * lane;  // bytes of this lane's word inside the row
+  const uint32_t keep = valid >= 4 ? ~0u : valid <= 0 ? 0u : (1u << (8 * valid)) - 1u;
+  const int64_t first = min(row0 + r0, rows - 1), last = min(row0 + r0 + (ROWS - 1) * step, rows - 1);
+  const uintptr_t from = reinterpret_cast<uintptr_t>(base + first * stride + at);
+  uint32_t v[ROWS];
+  if ((from & ~static_cast<uintptr_t>(3)) >= span.lo &&
+      reinterpret_cast<uintptr_t>(base + last * stride + at) + 128 + 4 <= span.hi) {  // the same for the whole warp
+    uint32_t low[ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const int64_t row = min(row0 + r0 + i * step, rows - 1);
+      const uint32_t* a = reinterpret_cast<const uint32_t*>(reinterpret_cast<uintptr_t>(base + row * stride + at) &
+                                                            ~static_cast<uintptr_t>(3)) + lane;
+      low[i] = a[0];
+      v[i] = a[1];
+    }
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const int64_t row = min(row0 + r0 + i * step, rows - 1);
+      v[i] = __funnelshift_r(low[i], v[i], 8 * (reinterpret_cast<uintptr_t>(base + row * stride + at) & 3));
+    }
+  } else {
+#pragma unroll 1
+    for (int i = 0; i < ROWS; ++i) {
+      const int64_t row = min(row0 + r0 + i * step, rows - 1);
+      uint32_t w = 0;
+      for (int b = 0; b < 4; ++b)
+        if (b < valid) w |= static_cast<uint32_t>(base[row * stride + at + 4 * lane + b]) << (8 * b);
+#pragma unroll
+      for (int j = 0; j < ROWS; ++j)
+        if (j == i) v[j] = w;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int r = r0 + i * step;
+    if (r < box_rows)
+      asm volatile("st.shared.u32 [%0], %1;" ::"r"(dst + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + 4 * (lane & 3)),
+                   "r"(row0 + r < rows ? v[i] & keep : 0u)
+                   : "memory");
+  }
+}
+
 // 4-bit weights as exact 16-bit floats: a nibble or'ed into the mantissa of 128 (bf16) or 1024 (f16).
 template <typename X>
 __host__ __device__ constexpr uint32_t nibble_magic();
