@@ -226,7 +226,7 @@ k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUte
 #pragma unroll 1
       for (int i = 0; i < 8; ++i) {
         uint32_t q[4];
-        load_bytes<16>(w, static_cast<int64_t>(kb) * (kBlockK / 2) + 16 * i, end, span, q);
+        load_bytes<16, false>(w, static_cast<int64_t>(kb) * (kBlockK / 2) + 16 * i, end, span, q);
         asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(own + slot * kChunkBytes + ((i ^ (r & 7)) << 4)),
                      "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3])
                      : "memory");

@@ -59,30 +59,28 @@ __global__ void __launch_bounds__(32 * kWarps) k_small_w4(const __grid_constant_
   const int64_t w_end = (p.k + 1) / 2;
   const Span span_w = span_of(p.w, p.n, p.w_stride, w_end), span_x = span_of(p.x, p.rows, 2 * p.x_stride, 2 * p.k);
   const int64_t groups = (p.k + GROUP - 1) / GROUP;
+  const uint8_t* x_row[NT];  // columns behind the last row of x repeat it and are not stored
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+    x_row[j] = static_cast<const uint8_t*>(p.x) + 2 * min(t0 + 8 * j + (lane >> 2), p.rows - 1) * p.x_stride;
   const Nibbles<X> nibbles;
   float acc[NT][4] = {};
-  for (int64_t g = warp; g < groups; g += kWarps) {
+  auto group_of = [&](int64_t g, auto inside) {
+    constexpr bool kInside = decltype(inside)::value;
     const int64_t k0 = g * GROUP + (lane & 3) * (GROUP / 4);
     uint32_t q[2][kWords], zero[2];
     float scale[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      load_bytes<kBytes>(w[h], k0 / 2, w_end, span_w, q[h]);
+      load_bytes<kBytes, kInside>(w[h], k0 / 2, w_end, span_w, q[h]);
       scale[h] = load_scale(p.scale4, p.scale_type, row[h] * p.scale_stride + g);
       const uint32_t z = p.zeros == nullptr ? 8u : p.zeros[row[h] * p.zeros_stride + g] & 15u;
       zero[h] = kMagic | z | (z << 16);
     }
     uint32_t x[NT][kWords][4];  // eight consecutive values of x for each word of weights
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const int64_t t = t0 + 8 * j + (lane >> 2);
-      if (t < p.rows) {
-        load_bytes<16 * kWords>(static_cast<const uint8_t*>(p.x) + 2 * t * p.x_stride, 2 * k0, 2 * p.k, span_x, &x[j][0][0]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4 * kWords; ++i) (&x[j][0][0])[i] = 0;
-      }
-    }
+    for (int j = 0; j < NT; ++j)
+      load_bytes<16 * kWords, kInside>(x_row[j], 2 * k0, 2 * p.k, span_x, &x[j][0][0]);
     float sum[NT][4] = {};
 #pragma unroll
     for (int i = 0; i < kWords; ++i) {
@@ -101,6 +99,11 @@ __global__ void __launch_bounds__(32 * kWarps) k_small_w4(const __grid_constant_
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[j][i] = fmaf(scale[i >> 1], sum[j][i], acc[j][i]);
+  };
+#pragma unroll 1
+  for (int64_t g = warp; g < groups; g += kWarps) {
+    if (g > 0 && (g + 1) * (GROUP / 2) + 4 <= w_end && (g + 1) * GROUP + 2 <= p.k) group_of(g, std::true_type());
+    else group_of(g, std::false_type());
   }
   fold<NT, float>(acc, p, n0, t0, [&](int64_t t, int64_t n, float v) { store_out(p.out, p.out_type, t * p.out_stride + n, v); });
 }
@@ -116,21 +119,18 @@ __global__ void __launch_bounds__(32 * kWarps) k_small_8(const __grid_constant__
     w[h] = static_cast<const uint8_t*>(p.w) + min(n0 + (lane >> 2) + 8 * h, p.n - 1) * p.w_stride;
   const Span span_w = span_of(p.w, p.n, p.w_stride, p.k), span_x = span_of(p.x, p.rows, p.x_stride, p.k);
   Acc acc[NT][4] = {};
-  for (int64_t c = warp; c * 64 < p.k; c += kWarps) {
+  const uint8_t* x_row[NT];  // columns behind the last row of x repeat it and are not stored
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+    x_row[j] = static_cast<const uint8_t*>(p.x) + min(t0 + 8 * j + (lane >> 2), p.rows - 1) * p.x_stride;
+  auto chunk = [&](int64_t c, auto inside) {
+    constexpr bool kInside = decltype(inside)::value;
     const int64_t k0 = c * 64 + (lane & 3) * 16;
     uint32_t q[2][4], x[NT][4];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) load_bytes<16>(w[h], k0, p.k, span_w, q[h]);
+    for (int h = 0; h < 2; ++h) load_bytes<16, kInside>(w[h], k0, p.k, span_w, q[h]);
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const int64_t t = t0 + 8 * j + (lane >> 2);
-      if (t < p.rows) {
-        load_bytes<16>(static_cast<const uint8_t*>(p.x) + t * p.x_stride, k0, p.k, span_x, x[j]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[j][i] = 0;
-      }
-    }
+    for (int j = 0; j < NT; ++j) load_bytes<16, kInside>(x_row[j], k0, p.k, span_x, x[j]);
     if constexpr (I8) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -151,6 +151,11 @@ __global__ void __launch_bounds__(32 * kWarps) k_small_8(const __grid_constant__
         for (int j = 0; j < NT; ++j) mma_f16(acc[j], a, wx[j][i][0], wx[j][i][1]);
       }
     }
+  };
+#pragma unroll 1
+  for (int64_t c = warp; c * 64 < p.k; c += kWarps) {
+    if (c > 0 && (c + 1) * 64 + 4 <= p.k) chunk(c, std::true_type());
+    else chunk(c, std::false_type());
   }
   fold<NT, Acc>(acc, p, n0, t0, [&](int64_t t, int64_t n, Acc v) {
     store_out(p.out, p.out_type, t * p.out_stride + n, static_cast<float>(v) * p.x_scale[t] * p.w_scale8[n]);

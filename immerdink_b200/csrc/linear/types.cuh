@@ -51,23 +51,22 @@ __device__ __forceinline__ Span span_of(const void* p, int64_t rows, int64_t str
   return {lo, lo + static_cast<uintptr_t>((rows - 1) * stride_bytes + row_bytes)};
 }
 
-// `BYTES` bytes at row + at, zeros from `end` (the row's length in bytes) on, for rows of any alignment: they
-// are read as the aligned words around them, shifted into place, wherever those words lie inside the matrix;
-// single bytes remain at its two ends and at a row's end.
-template <int BYTES>
+// `BYTES` bytes at row + at, zeros from `end` (the row's length in bytes) on, for rows of any alignment. INSIDE: the
+// piece lies inside the row with at least 3 bytes before and 4 behind it, and is read as the aligned words around it,
+// shifted into place, without a branch (so that many such loads are in flight together). Otherwise the same where
+// those words lie inside the matrix, and single bytes elsewhere.
+template <int BYTES, bool INSIDE>
 __device__ __forceinline__ void load_bytes(const uint8_t* row, int64_t at, int64_t end, const Span& span, uint32_t* v) {
   const uint8_t* p = row + at;
   const uintptr_t first = reinterpret_cast<uintptr_t>(p) & ~static_cast<uintptr_t>(3);
-  if (at + BYTES <= end && first >= span.lo && first + BYTES + 4 <= span.hi) {
+  if (INSIDE || (at + BYTES <= end && first >= span.lo && first + BYTES + 4 <= span.hi)) {
     const uint32_t shift = 8 * (reinterpret_cast<uintptr_t>(p) & 3);
     const uint32_t* q = reinterpret_cast<const uint32_t*>(first);
-    uint32_t low = q[0];
+    uint32_t word[BYTES / 4 + 1];
 #pragma unroll
-    for (int i = 0; i < BYTES / 4; ++i) {
-      const uint32_t high = q[i + 1];
-      v[i] = __funnelshift_r(low, high, shift);
-      low = high;
-    }
+    for (int i = 0; i <= BYTES / 4; ++i) word[i] = q[i];
+#pragma unroll
+    for (int i = 0; i < BYTES / 4; ++i) v[i] = __funnelshift_r(word[i], word[i + 1], shift);
     return;
   }
 #pragma unroll
