@@ -25,7 +25,7 @@
 namespace imd {
 namespace {
 
-constexpr int kThreads = 192;       // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue
+constexpr int kThreads = 320;       // warp 0 TMA, warp 1 MMA, warps 2-9 epilogue
 constexpr int kTileM = 128;         // rows of one CTA's accumulator
 constexpr int kTileK = 128;         // bytes of K per pipeline stage = one swizzle row
 constexpr int kMmaK = 32;
@@ -71,28 +71,54 @@ __device__ __forceinline__ float acc_value(uint32_t v) {
   return I8 ? static_cast<float>(static_cast<int32_t>(v)) : __uint_as_float(v);
 }
 
-template <typename T>
-__device__ __forceinline__ void store_wide(void* out, int64_t i, const float* v) {
-  constexpr int V = 16 / sizeof(T);
+// 32 columns of a warp's 32 rows (lane = row) to output rows in 16-byte units: 64 bytes of each row at a time go
+// through shared memory (pitch 80 bytes: no bank conflicts), so that a store covers 64 bytes of 8 rows and not 16 bytes
+// of 32. `at` is the element of lane 0's row; `rows` how many of the warp's rows exist.
+template <bool I8, typename T>
+__device__ __forceinline__ void store_block(const Params& p, int64_t at, int rows, const uint32_t* v, float xs, const float* ws,
+                                            uint8_t* turn, int lane) {
+  constexpr int kCols = 64 / sizeof(T), V = 16 / sizeof(T);
 #pragma unroll
-  for (int c = 0; c < 16; c += V) {
-    Pack<T, V> o;
+  for (int h = 0; h < 32; h += kCols) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) o.v[j] = from_float<T>(v[c + j]);
-    *reinterpret_cast<Pack<T, V>*>(static_cast<T*>(out) + i + c) = o;
+    for (int c = 0; c < kCols; c += V) {
+      Pack<T, V> o;
+#pragma unroll
+      for (int j = 0; j < V; ++j) o.v[j] = from_float<T>(acc_value<I8>(v[h + c + j]) * xs * ws[h + c + j]);
+      *reinterpret_cast<uint4*>(turn + lane * 80 + c * sizeof(T)) = *reinterpret_cast<const uint4*>(&o);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 8 * i + (lane >> 2);
+      if (r < rows)
+        *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + at + r * p.out_stride + h + (lane & 3) * V) =
+            *reinterpret_cast<const uint4*>(turn + r * 80 + (lane & 3) * 16);
+    }
+    __syncwarp();
   }
+}
+// Sixteen columns of 32 turned rows: lane l has column l mod 16 and every second row from l / 16 on.
+template <typename T>
+__device__ __forceinline__ void store_turned(const Params& p, int64_t at, int rows, const float* turn, int lane, float scale) {
+  T* out = static_cast<T*>(p.out) + at;
+  const float* from = turn + (lane >> 4) * 17 + (lane & 15);
+#pragma unroll
+  for (int r = 0; r < 32; r += 2, out += 2 * p.out_stride, from += 34)
+    if (r < rows) *out = from_float<T>(*from * scale);
 }
 
 // ---- many rows: CTA pairs ------------------------------------------------------------------------------
 // Signals as in the contraction's pair kernel: full[s] in the leader, armed with the bytes of both CTAs;
-// empty[s] and tfull[a] by commits that reach both CTAs; tempty[a] in the leader, eight epilogue warps.
-constexpr int kTurnBytes = 32 * 33 * 4;  // a warp's 32 x 32 block, turned for stores along the rows
+// empty[s] and tfull[a] by commits that reach both CTAs; tempty[a] in the leader, the sixteen epilogue
+// warps of both.
+constexpr int kTurnBytes = 32 * 80;  // a warp's block on its way to stores along the rows
 template <int BN>
 constexpr int kPairStageBytes = kBytesM + BN / 2 * kTileK;
 template <int BN>
 constexpr int kPairStages = BN == 256 ? 6 : 8;
 template <int BN>
-constexpr int kPairSmem = kPairStages<BN> * kPairStageBytes<BN> + 1024 + kCtrlBytes + 4 * kTurnBytes;
+constexpr int kPairSmem = kPairStages<BN> * kPairStageBytes<BN> + 1024 + kCtrlBytes + 8 * kTurnBytes + 2 * BN * 4;
 
 __device__ __forceinline__ void pair_tile(const Params& p, int w, int* tm, int* tn) {
   const int band = p.band_rows * p.tiles_n;
@@ -132,7 +158,7 @@ k_dense8_pair(const __grid_constant__ CUtensorMap map_x, const __grid_constant__
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(tfull(a), 1);
-      mbar_init(tempty(a), 8);
+      mbar_init(tempty(a), 16);
     }
     mbar_init(drain, 1);
     *abort = 0;
@@ -153,6 +179,7 @@ k_dense8_pair(const __grid_constant__ CUtensorMap map_x, const __grid_constant__
   const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
   const uint32_t peer_abort = map_to_cta(smem_u32(const_cast<int*>(abort)), rank ^ 1u);
   auto tell_peer = [&]() { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(peer_abort), "r"(1u) : "memory"); };
+  bool gave_up = false;  // of an epilogue warp
 
   if (warp == 0) {
     if (lane == 0) {
@@ -227,51 +254,58 @@ k_dense8_pair(const __grid_constant__ CUtensorMap map_x, const __grid_constant__
         if (mbar_try_wait(drain, 0)) break;
     }
   } else {
-    const int quarter = warp & 3;
+    // two warps per quarter of the tensor memory's lanes take the columns by turns of 32
+    const int quarter = warp & 3, first_col = warp < 6 ? 0 : 32, id = static_cast<int>(threadIdx.x) - 64;
+    float* turn = reinterpret_cast<float*>(ctrl + kCtrlBytes) + (warp - 2) * (kTurnBytes / 4);
+    float* scales = reinterpret_cast<float*>(ctrl + kCtrlBytes + 8 * kTurnBytes);
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int w = first; w < total; w += step) {
       int tm, tn;
       pair_tile(p, w, &tm, &tn);
+      // the columns' scales to shared memory, in the half that the tile before last used
+      float* ws = scales + acc * BN;
+      if (id < BN) ws[id] = tn * BN + id < p.n ? p.w_scale[tn * BN + id] : 0.0f;
+      asm volatile("bar.sync 1, 256;" ::: "memory");
       if (!mbar_wait(tfull(acc), acc_phase, abort)) {
         if (lane == 0) tell_peer();
-        break;
+        // the other warps of the CTA give up at their own wait: every one of them passes the barrier above
+        gave_up = true;
       }
+      __syncwarp();
       tc_fence_after();
       const int row = tm * 256 + static_cast<int>(rank) * 128 + quarter * 32 + lane;
       const float xs = row < p.rows ? p.x_scale[row] : 0.0f;
-      const int64_t base = static_cast<int64_t>(row) * p.out_stride;
       const uint32_t taddr = tmem_base + acc * BN + (static_cast<uint32_t>(quarter * 32) << 16);
-      float* turn = reinterpret_cast<float*>(ctrl + kCtrlBytes) + (warp - 2) * (kTurnBytes / 4);
 #pragma unroll 1
-      for (int cc = 0; cc < BN; cc += 32) {
+      for (int cc = first_col; cc < BN && !gave_up; cc += 64) {
         const int col = tn * BN + cc;
         if (col >= p.n) break;  // the same for the whole warp
         uint32_t v[32];
         tmem_load_32(taddr + cc, v);
         if (p.out_wide && col + 32 <= p.n) {  // the same for the whole warp
-          if (row < p.rows) {
-#pragma unroll
-            for (int h = 0; h < 32; h += 16) {
-              float f[16];
-#pragma unroll
-              for (int j = 0; j < 16; ++j) f[j] = acc_value<I8>(v[h + j]) * xs * __ldg(p.w_scale + col + h + j);
-              if (p.out_type == IMD_TYPE_F32) store_wide<float>(p.out, base + col + h, f);
-              else if (p.out_type == IMD_TYPE_F16) store_wide<__half>(p.out, base + col + h, f);
-              else store_wide<__nv_bfloat16>(p.out, base + col + h, f);
-            }
-          }
+          const int64_t at = static_cast<int64_t>(row - lane) * p.out_stride + col;
+          uint8_t* block = reinterpret_cast<uint8_t*>(turn);
+          if (p.out_type == IMD_TYPE_F32) store_block<I8, float>(p, at, p.rows - (row - lane), v, xs, ws + cc, block, lane);
+          else if (p.out_type == IMD_TYPE_F16) store_block<I8, __half>(p, at, p.rows - (row - lane), v, xs, ws + cc, block, lane);
+          else store_block<I8, __nv_bfloat16>(p, at, p.rows - (row - lane), v, xs, ws + cc, block, lane);
         } else {
-          // rows of the output that start anywhere: the block is turned in shared memory so that a
-          // warp stores 32 neighbours of one row (a lane's own row would touch 32 sectors a store)
+          // rows of the output that start anywhere: blocks are turned in shared memory so that a warp stores 16
+          // neighbours of two rows (a lane's own row would touch 32 sectors a store)
 #pragma unroll
-          for (int j = 0; j < 32; ++j) turn[lane * 33 + j] = acc_value<I8>(v[j]) * xs;
-          __syncwarp();
-          const float ws = col + lane < p.n ? p.w_scale[col + lane] : 0.0f;
-          const int rows = min(32, p.rows - (row - lane));
-          for (int r = 0; r < rows; ++r)
-            if (col + lane < p.n)
-              store_out(p.out, p.out_type, static_cast<int64_t>(row - lane + r) * p.out_stride + col + lane, turn[r * 33 + lane] * ws);
+          for (int h = 0; h < 32; h += 16) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) turn[lane * 17 + j] = acc_value<I8>(v[h + j]) * xs;
+            __syncwarp();
+            const int c = col + h + (lane & 15);
+            const int64_t at = static_cast<int64_t>(row - lane + (lane >> 4)) * p.out_stride + c;
+            const int rows = c < p.n ? p.rows - (row - lane + (lane >> 4)) : 0;
+            const float scale = ws[cc + h + (lane & 15)];
+            if (p.out_type == IMD_TYPE_F32) store_turned<float>(p, at, rows, turn, lane, scale);
+            else if (p.out_type == IMD_TYPE_F16) store_turned<__half>(p, at, rows, turn, lane, scale);
+            else store_turned<__nv_bfloat16>(p, at, rows, turn, lane, scale);
+            __syncwarp();
+          }
         }
         __syncwarp();
       }
@@ -293,7 +327,6 @@ k_dense8_pair(const __grid_constant__ CUtensorMap map_x, const __grid_constant__
 }
 
 // ---- up to 256 rows: weights on the M side ---------------------------------------------------------------
-constexpr int kSwapThreads = 320;  // warp 0 TMA, warp 1 MMA, warps 2-9 epilogue
 constexpr int kSwapMaxStages = 12;
 
 __device__ __forceinline__ uint32_t load_cluster(uint32_t addr) {
@@ -372,7 +405,7 @@ __device__ __forceinline__ void swap_epilogue(const Params& p, uint32_t tmem_bas
 // ANY: rows that TMA cannot bring. The epilogue's warps, idle until the sums are complete, bring the operands'
 // next 128 bytes per row instead, row by row.
 template <bool I8, bool ANY>
-__global__ void __launch_bounds__(kSwapThreads)
+__global__ void __launch_bounds__(kThreads)
 k_dense8_swap(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
               const __grid_constant__ Params call) {
   Params p = call;
@@ -401,7 +434,7 @@ k_dense8_swap(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
   const int kb1 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * (part + 1) / parts);
   const int n0 = blockIdx.x * kTileM;
   __shared__ float x_scale[256];
-  for (int i = threadIdx.x; i < p.cols; i += kSwapThreads) x_scale[i] = i < p.rows ? p.x_scale[i] : 0.0f;
+  for (int i = threadIdx.x; i < p.cols; i += kThreads) x_scale[i] = i < p.rows ? p.x_scale[i] : 0.0f;
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) {
       mbar_init(full(s), ANY ? 8 : 1);
@@ -555,7 +588,7 @@ bool launch_swap(const LinearArgs& a, const DeviceInfo& dev, Params p, cudaStrea
   if (static_cast<int64_t>(p.stages) * stage_bytes < static_cast<int64_t>(p.cols) * kTileM * 4) return false;  // (the fold)
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned int>(tiles), static_cast<unsigned int>(parts), static_cast<unsigned int>(tiles_z));
-  cfg.blockDim = dim3(kSwapThreads);
+  cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = static_cast<size_t>(p.stages) * stage_bytes + 1024 + kCtrlBytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -586,7 +619,7 @@ bool launch(const LinearArgs& a, const DeviceInfo& dev, const Params& p, cudaStr
   // narrower tile costs
   const int64_t tiles_m = (a.rows + 255) / 256, pairs = dev.sms / 2;
   auto waves = [&](int64_t bn) { return (tiles_m * ((a.n + bn - 1) / bn) + pairs - 1) / pairs * bn; };
-  if (waves(128) * 115 < waves(256) * 100) return launch_pair<I8, 128>(a, dev, p, stream);
+  if (waves(128) * 125 < waves(256) * 100) return launch_pair<I8, 128>(a, dev, p, stream);
   return launch_pair<I8, 256>(a, dev, p, stream);
 }
 
