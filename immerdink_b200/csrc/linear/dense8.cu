@@ -71,12 +71,13 @@ __device__ __forceinline__ float acc_value(uint32_t v) {
   return I8 ? static_cast<float>(static_cast<int32_t>(v)) : __uint_as_float(v);
 }
 
-// 32 columns of a warp's 32 rows (lane = row) to output rows in 16-byte units: 64 bytes of each row at a time go
-// through shared memory (pitch 80 bytes: no bank conflicts), so that a store covers 64 bytes of 8 rows and not 16 bytes
-// of 32. `at` is the element of lane 0's row; `rows` how many of the warp's rows exist.
-template <bool I8, typename T>
-__device__ __forceinline__ void store_block(const Params& p, int64_t at, int rows, const uint32_t* v, float xs, const float* ws,
-                                            uint8_t* turn, int lane) {
+// 32 columns of a warp's 32 rows (lane = row) to output rows, by way of shared memory: 64 bytes of each row at a time
+// (pitch 80 bytes: no bank conflicts), so that a store covers neighbours. WIDE: 16-byte units, 64 bytes of 8 rows a
+// store instead of 16 bytes of 32. Otherwise rows that start anywhere and the columns of the last tile, an element per
+// lane. `at` is the element of lane 0's row; `rows` and `cols` how many of the block exist.
+template <bool I8, typename T, bool WIDE>
+__device__ __forceinline__ void store_block(const Params& p, int64_t at, int rows, int cols, const uint32_t* v, float xs,
+                                            const float* ws, uint8_t* turn, int lane) {
   constexpr int kCols = 64 / sizeof(T), V = 16 / sizeof(T);
 #pragma unroll
   for (int h = 0; h < 32; h += kCols) {
@@ -88,24 +89,31 @@ __device__ __forceinline__ void store_block(const Params& p, int64_t at, int row
       *reinterpret_cast<uint4*>(turn + lane * 80 + c * sizeof(T)) = *reinterpret_cast<const uint4*>(&o);
     }
     __syncwarp();
+    if (WIDE) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = 8 * i + (lane >> 2);
-      if (r < rows)
-        *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + at + r * p.out_stride + h + (lane & 3) * V) =
-            *reinterpret_cast<const uint4*>(turn + r * 80 + (lane & 3) * 16);
+      for (int i = 0; i < 4; ++i) {
+        const int r = 8 * i + (lane >> 2);
+        if (r < rows)
+          *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + at + r * p.out_stride + h + (lane & 3) * V) =
+              *reinterpret_cast<const uint4*>(turn + r * 80 + (lane & 3) * 16);
+      }
+    } else {
+      constexpr int kRowsAtOnce = 32 / kCols;  // of a store
+      const int c = lane % kCols, r0 = lane / kCols, last = h + c < cols ? rows : 0;
+      T* out = static_cast<T*>(p.out) + at + r0 * p.out_stride + h + c;
+      const T* from = reinterpret_cast<const T*>(turn + r0 * 80) + c;
+#pragma unroll
+      for (int r = 0; r < 32; r += kRowsAtOnce, out += kRowsAtOnce * p.out_stride)
+        if (r0 + r < last) *out = from[r * (80 / sizeof(T))];
     }
     __syncwarp();
   }
 }
-// Sixteen columns of 32 turned rows: lane l has column l mod 16 and every second row from l / 16 on.
-template <typename T>
-__device__ __forceinline__ void store_turned(const Params& p, int64_t at, int rows, const float* turn, int lane, float scale) {
-  T* out = static_cast<T*>(p.out) + at;
-  const float* from = turn + (lane >> 4) * 17 + (lane & 15);
-#pragma unroll
-  for (int r = 0; r < 32; r += 2, out += 2 * p.out_stride, from += 34)
-    if (r < rows) *out = from_float<T>(*from * scale);
+template <bool I8, typename T>
+__device__ __forceinline__ void store_block(const Params& p, int64_t at, int rows, int cols, const uint32_t* v, float xs,
+                                            const float* ws, uint8_t* turn, int lane) {
+  if (p.out_wide && cols >= 32) store_block<I8, T, true>(p, at, rows, cols, v, xs, ws, turn, lane);
+  else store_block<I8, T, false>(p, at, rows, cols, v, xs, ws, turn, lane);
 }
 
 // ---- many rows: CTA pairs ------------------------------------------------------------------------------
@@ -256,7 +264,7 @@ k_dense8_pair(const __grid_constant__ CUtensorMap map_x, const __grid_constant__
   } else {
     // two warps per quarter of the tensor memory's lanes take the columns by turns of 32
     const int quarter = warp & 3, first_col = warp < 6 ? 0 : 32, id = static_cast<int>(threadIdx.x) - 64;
-    float* turn = reinterpret_cast<float*>(ctrl + kCtrlBytes) + (warp - 2) * (kTurnBytes / 4);
+    uint8_t* turn = ctrl + kCtrlBytes + (warp - 2) * kTurnBytes;
     float* scales = reinterpret_cast<float*>(ctrl + kCtrlBytes + 8 * kTurnBytes);
     int acc = 0;
     uint32_t acc_phase = 0;
@@ -283,30 +291,11 @@ k_dense8_pair(const __grid_constant__ CUtensorMap map_x, const __grid_constant__
         if (col >= p.n) break;  // the same for the whole warp
         uint32_t v[32];
         tmem_load_32(taddr + cc, v);
-        if (p.out_wide && col + 32 <= p.n) {  // the same for the whole warp
-          const int64_t at = static_cast<int64_t>(row - lane) * p.out_stride + col;
-          uint8_t* block = reinterpret_cast<uint8_t*>(turn);
-          if (p.out_type == IMD_TYPE_F32) store_block<I8, float>(p, at, p.rows - (row - lane), v, xs, ws + cc, block, lane);
-          else if (p.out_type == IMD_TYPE_F16) store_block<I8, __half>(p, at, p.rows - (row - lane), v, xs, ws + cc, block, lane);
-          else store_block<I8, __nv_bfloat16>(p, at, p.rows - (row - lane), v, xs, ws + cc, block, lane);
-        } else {
-          // rows of the output that start anywhere: blocks are turned in shared memory so that a warp stores 16
-          // neighbours of two rows (a lane's own row would touch 32 sectors a store)
-#pragma unroll
-          for (int h = 0; h < 32; h += 16) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) turn[lane * 17 + j] = acc_value<I8>(v[h + j]) * xs;
-            __syncwarp();
-            const int c = col + h + (lane & 15);
-            const int64_t at = static_cast<int64_t>(row - lane + (lane >> 4)) * p.out_stride + c;
-            const int rows = c < p.n ? p.rows - (row - lane + (lane >> 4)) : 0;
-            const float scale = ws[cc + h + (lane & 15)];
-            if (p.out_type == IMD_TYPE_F32) store_turned<float>(p, at, rows, turn, lane, scale);
-            else if (p.out_type == IMD_TYPE_F16) store_turned<__half>(p, at, rows, turn, lane, scale);
-            else store_turned<__nv_bfloat16>(p, at, rows, turn, lane, scale);
-            __syncwarp();
-          }
-        }
+        const int64_t at = static_cast<int64_t>(row - lane) * p.out_stride + col;
+        const int rows = p.rows - (row - lane), cols = p.n - col;
+        if (p.out_type == IMD_TYPE_F32) store_block<I8, float>(p, at, rows, cols, v, xs, ws + cc, turn, lane);
+        else if (p.out_type == IMD_TYPE_F16) store_block<I8, __half>(p, at, rows, cols, v, xs, ws + cc, turn, lane);
+        else store_block<I8, __nv_bfloat16>(p, at, rows, cols, v, xs, ws + cc, turn, lane);
         __syncwarp();
       }
       tc_fence_before();
