@@ -39,8 +39,10 @@ bool encode_rows_128(const DeviceInfo& dev, CUtensorMap* map, const void* base, 
   const cuuint32_t box[3] = {128, static_cast<cuuint32_t>(box_rows), 1};
   const cuuint32_t elem[3] = {1, 1, 1};
   const EncodeTiled fn = reinterpret_cast<EncodeTiled>(dev.encode_tiled);
+  // rows that straddle the 128-byte lines cost more with larger fetches (e4m3 1999 x 5003 x 4176: 63 against 58 us)
+  const CUtensorMapL2promotion fetch = pitch % 128 == 0 ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_NONE;
   return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, elem,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, fetch,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
