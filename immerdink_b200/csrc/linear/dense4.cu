@@ -304,7 +304,7 @@ k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUte
       return g < groups ? load_scale(p.a.scale4, p.a.scale_type, nc * p.a.scale_stride + g) : 0.0f;
     };
     // four groups' scales are loaded four groups ahead. The loop over the groups stays rolled: the roles' hot
-    // loops together have to fit the instruction cache (unrolled by four they did not: 400 against TODO us)
+    // loops together have to fit the instruction cache (unrolled by four: 400 against 376 us at 2048 x 8192 x 8192)
     const int g0 = u0 * kGroups;
     float scale[4], next[4];
 #pragma unroll

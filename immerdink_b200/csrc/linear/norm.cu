@@ -71,6 +71,17 @@ struct Piece {
       w[0] = *reinterpret_cast<const uint16_t*>(at);
     }
   }
+  // The first n elements (at most V), one by one; zeros behind them.
+  __device__ __forceinline__ void load_part(const void* p, int64_t i, int n) {
+    clear();
+    const T* at = static_cast<const T*>(p) + i;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      if (v >= n) continue;
+      if constexpr (sizeof(T) == 4) w[v] = reinterpret_cast<const uint32_t*>(at)[v];
+      else w[v / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(at)[v]) << (16 * (v & 1));
+    }
+  }
   __device__ __forceinline__ float value(int v) const {
     if constexpr (sizeof(T) == 4) {
       return __uint_as_float(w[v]);
@@ -104,16 +115,14 @@ struct Piece {
   }
 };
 
-// V codes of the scaled values y. int8: adding 1.5 * 2^23 rounds to the nearest even integer and leaves it,
-// in two's complement, in the low bits; `keep` clears the codes of a row that has no finite scale.
+// V codes of the scaled values y as bytes of words. int8: adding 1.5 * 2^23 rounds to the nearest even integer and
+// leaves it, in two's complement, in the low bits; `keep` clears the codes of a row that has no finite scale.
 template <int V>
-__device__ __forceinline__ void store_codes(void* p, int64_t i, const float* y, bool e4m3, uint32_t keep) {
-  uint8_t* at = static_cast<uint8_t*>(p) + i;
+__device__ __forceinline__ void codes(const float* y, bool e4m3, uint32_t keep, uint32_t* o) {
   if constexpr (V == 1) {
-    *at = e4m3 ? static_cast<uint8_t>(__nv_cvt_float_to_fp8(y[0], __NV_SATFINITE, __NV_E4M3))
-               : static_cast<uint8_t>(__float_as_uint(y[0] + 12582912.0f) & keep);
+    o[0] = e4m3 ? static_cast<uint32_t>(__nv_cvt_float_to_fp8(y[0], __NV_SATFINITE, __NV_E4M3))
+                : __float_as_uint(y[0] + 12582912.0f) & keep;
   } else {
-    uint32_t o[V / 4];
 #pragma unroll
     for (int j = 0; j < V / 4; ++j) {
       const float* f = y + 4 * j;
@@ -128,9 +137,66 @@ __device__ __forceinline__ void store_codes(void* p, int64_t i, const float* y, 
         o[j] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410) & keep;
       }
     }
-    if constexpr (V == 8) *reinterpret_cast<uint2*>(at) = make_uint2(o[0], o[1]);
-    else *reinterpret_cast<uint32_t*>(at) = o[0];
   }
+}
+template <int V>
+__device__ __forceinline__ void store_codes(void* p, int64_t i, const float* y, bool e4m3, uint32_t keep) {
+  uint8_t* at = static_cast<uint8_t*>(p) + i;
+  uint32_t o[V < 4 ? 1 : V / 4];
+  codes<V>(y, e4m3, keep, o);
+  if constexpr (V == 8) *reinterpret_cast<uint2*>(at) = make_uint2(o[0], o[1]);
+  else if constexpr (V == 4) *reinterpret_cast<uint32_t*>(at) = o[0];
+  else *at = static_cast<uint8_t>(o[0]);
+}
+
+// `bytes` bytes of words to an address of any alignment that is the same for the whole warp modulo 4: as many
+// aligned words as there are, halves and bytes around them.
+template <int WORDS>
+__device__ __forceinline__ void store_bytes(uint8_t* at, const uint32_t* o, int bytes) {
+  if (bytes < 4 * WORDS) {
+#pragma unroll
+    for (int i = 0; i < 4 * WORDS; ++i)
+      if (i < bytes) at[i] = static_cast<uint8_t>(o[i / 4] >> (8 * (i & 3)));
+    return;
+  }
+  const int head = static_cast<int>(-reinterpret_cast<uintptr_t>(at) & 3);  // bytes before the first aligned word
+  if (head == 0) {
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) reinterpret_cast<uint32_t*>(at)[i] = o[i];
+    return;
+  }
+  if (head & 1) *at = static_cast<uint8_t>(o[0]);
+  if (head & 2) *reinterpret_cast<uint16_t*>(at + (head & 1)) = static_cast<uint16_t>(o[0] >> (8 * (head & 1)));
+#pragma unroll
+  for (int i = 0; i + 1 < WORDS; ++i) *reinterpret_cast<uint32_t*>(at + head + 4 * i) = __funnelshift_r(o[i], o[i + 1], 8 * head);
+  const uint32_t tail = o[WORDS - 1] >> (8 * head);  // 4 - head bytes
+  uint8_t* end = at + 4 * WORDS - (4 - head);
+  if (head == 3) {
+    *end = static_cast<uint8_t>(tail);
+  } else {
+    *reinterpret_cast<uint16_t*>(end) = static_cast<uint16_t>(tail);
+    if (head == 1) end[2] = static_cast<uint8_t>(tail >> 16);
+  }
+}
+template <int V>
+__device__ __forceinline__ void store_codes_any(uint8_t* at, const float* y, int n, bool e4m3, uint32_t keep) {
+  uint32_t o[V / 4];
+  codes<V>(y, e4m3, keep, o);
+  if (n > 0) store_bytes<V / 4>(at, o, n);
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_any(T* at, const float* f, int n) {
+  uint32_t o[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (sizeof(T) == 4) {
+      o[j] = __float_as_uint(f[j]);
+    } else {
+      Pack<T, 2> h{{from_float<T>(f[2 * j]), from_float<T>(f[2 * j + 1])}};
+      o[j] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+  if (n > 0) store_bytes<4>(reinterpret_cast<uint8_t*>(at), o, n < V ? n * static_cast<int>(sizeof(T)) : 16);
 }
 
 // What turns a row's y into codes: q = round(y * pre * inv), scale as stored.
@@ -224,92 +290,96 @@ __global__ void __launch_bounds__(1024) k_norm_quantize_long(const __grid_consta
 }
 
 // From the 32-bit sums h of a row to its outputs; E vectors of V elements per thread. `loaded` is called once,
-// after the first reduction: every thread of the row has then taken its h from wherever the row was.
-template <typename T, int V, int E, bool WARP, typename Loaded>
+// after the first reduction: every thread of the row has then taken its h from wherever the row was. ANY: rows, weight
+// and outputs of any alignment, the last vector of a row may be short (its h are zeros).
+template <typename T, int V, int E, bool WARP, bool ANY, typename Loaded>
 __device__ __forceinline__ void finish_row(const NormArgs& p, int64_t row, int threads, int t, float (*h)[V], Shared& s,
                                            Loaded loaded) {
   const int dim = static_cast<int>(p.dim);
   const bool e4m3 = p.q_type == IMD_TYPE_E4M3, same = p.weight_type == p.x_type;
   Piece<T, V> w[E];
-      if (p.residual_out != nullptr) {
-        T* out = static_cast<T*>(p.residual_out) + row * p.residual_out_stride;
-  #pragma unroll
-        for (int i = 0; i < E; ++i) {
-          const int j = (i * threads + t) * V;
-          if (j < dim) Piece<T, V>::store(out, j, h[i]);
-        }
-      }
-      if (same) {
-  #pragma unroll
-        for (int i = 0; i < E; ++i) {
-          const int j = (i * threads + t) * V;
-          w[i].clear();
-          if (j < dim) w[i].load(p.weight, j);
-        }
-      }
-      float r;
-      for (uint32_t top = ~0u, e = 0;;) {  // a second time only for rows that leave the range
-        float ss = 0.0f;
-  #pragma unroll
-        for (int i = 0; i < E; ++i)
-  #pragma unroll
-          for (int v = 0; v < V; ++v) ss = fmaf(h[i][v], h[i][v], ss);
-        ss = row_sum<WARP>(ss, s.sums[top == ~0u ? 0 : 1]);
+  if (p.residual_out != nullptr) {
+    T* out = static_cast<T*>(p.residual_out) + row * p.residual_out_stride;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const int j = (i * threads + t) * V;
+      if constexpr (ANY) store_any<T, V>(out + j, h[i], dim - j);
+      else if (j < dim) Piece<T, V>::store(out, j, h[i]);
+    }
+  }
+  if (same) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const int j = (i * threads + t) * V;
+      w[i].clear();
+      if (ANY && (j + V > dim || reinterpret_cast<uintptr_t>(p.weight) % 16 != 0)) w[i].load_part(p.weight, j, dim - j);
+      else if (j < dim) w[i].load(p.weight, j);
+    }
+  }
+  float r;
+  for (uint32_t top = ~0u, e = 0;;) {  // a second time only for rows that leave the range
+    float ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+#pragma unroll
+      for (int v = 0; v < V; ++v) ss = fmaf(h[i][v], h[i][v], ss);
+    ss = row_sum<WARP>(ss, s.sums[top == ~0u ? 0 : 1]);
     if (top == ~0u) loaded();
-        const float mean = ss / static_cast<float>(dim);
-        if (top != ~0u) {
-          r = root_down(mean, p.eps_root, top, static_cast<int>(e));
-          break;
-        }
-        if (in_range(ss, p.eps)) {
-          r = 1.0f / sqrtf(mean + p.eps);
-          break;
-        }
-        top = 0;
-  #pragma unroll
-        for (int i = 0; i < E; ++i)
-  #pragma unroll
-          for (int v = 0; v < V; ++v) top = max(top, magnitude(h[i][v]));
-        top = row_max<WARP>(top, s.tops[0]);
-        if (top != 0 && top < 0x7F800000u) {
-          const Down d = scale_down(top);
-          e = static_cast<uint32_t>(d.e);
-  #pragma unroll
-          for (int i = 0; i < E; ++i)
-  #pragma unroll
-            for (int v = 0; v < V; ++v) h[i][v] = h[i][v] * d.f1 * d.f2;
-        }
-      }
-      uint32_t top = 0;
-      if (same) {
-  #pragma unroll
-        for (int i = 0; i < E; ++i)
-  #pragma unroll
-          for (int v = 0; v < V; ++v) h[i][v] = h[i][v] * r * w[i].value(v);
-      } else {
-  #pragma unroll
-        for (int i = 0; i < E; ++i) {
-          const int j = (i * threads + t) * V;
-  #pragma unroll
-          for (int v = 0; v < V; ++v)
-            if (j < dim) h[i][v] = h[i][v] * r * static_cast<const float*>(p.weight)[j + v];
-        }
-      }
-  #pragma unroll
+    const float mean = ss / static_cast<float>(dim);
+    if (top != ~0u) {
+      r = root_down(mean, p.eps_root, top, static_cast<int>(e));
+      break;
+    }
+    if (in_range(ss, p.eps)) {
+      r = 1.0f / sqrtf(mean + p.eps);
+      break;
+    }
+    top = 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+#pragma unroll
+      for (int v = 0; v < V; ++v) top = max(top, magnitude(h[i][v]));
+    top = row_max<WARP>(top, s.tops[0]);
+    if (top != 0 && top < 0x7F800000u) {
+      const Down d = scale_down(top);
+      e = static_cast<uint32_t>(d.e);
+#pragma unroll
       for (int i = 0; i < E; ++i)
-  #pragma unroll
-        for (int v = 0; v < V; ++v) top = max(top, magnitude(h[i][v]));
-      const RowScale c = row_scale(row_max<WARP>(top, s.tops[1]), e4m3 ? 448.0f : 127.0f);
-  #pragma unroll
-      for (int i = 0; i < E; ++i) {
-        const int j = (i * threads + t) * V;
-        if (j < dim) {
-  #pragma unroll
-          for (int v = 0; v < V; ++v) h[i][v] = h[i][v] * c.pre * c.inv;
-          store_codes<V>(static_cast<uint8_t*>(p.q) + row * p.q_stride, j, h[i], e4m3, c.keep);
-        }
-      }
-      if (t == 0) p.scale[row] = c.scale;
+#pragma unroll
+        for (int v = 0; v < V; ++v) h[i][v] = h[i][v] * d.f1 * d.f2;
+    }
+  }
+  uint32_t top = 0;
+  if (same) {
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+#pragma unroll
+      for (int v = 0; v < V; ++v) h[i][v] = h[i][v] * r * w[i].value(v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const int j = (i * threads + t) * V;
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (j + v < dim) h[i][v] = h[i][v] * r * static_cast<const float*>(p.weight)[j + v];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < E; ++i)
+#pragma unroll
+    for (int v = 0; v < V; ++v) top = max(top, magnitude(h[i][v]));
+  const RowScale c = row_scale(row_max<WARP>(top, s.tops[1]), e4m3 ? 448.0f : 127.0f);
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const int j = (i * threads + t) * V;
+    if (j < dim) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) h[i][v] = h[i][v] * c.pre * c.inv;
+      if constexpr (ANY) store_codes_any<V>(static_cast<uint8_t*>(p.q) + row * p.q_stride + j, h[i], dim - j, e4m3, c.keep);
+      else store_codes<V>(static_cast<uint8_t*>(p.q) + row * p.q_stride, j, h[i], e4m3, c.keep);
+    }
+  }
+  if (t == 0) p.scale[row] = c.scale;
 }
 
 // Rows in registers, one per warp or per CTA.
@@ -352,7 +422,7 @@ k_norm_quantize(const __grid_constant__ NormArgs p) {
 #pragma unroll
         for (int v = 0; v < V; ++v) h[i][v] += res[i].value(v);
     }
-    finish_row<T, V, E, WARP>(p, row, threads, t, h, s, [] {});
+    finish_row<T, V, E, WARP, false>(p, row, threads, t, h, s, [] {});
   }
 }
 
@@ -412,7 +482,7 @@ __global__ void __launch_bounds__(512, 2) k_norm_quantize_ring(const __grid_cons
         for (int v = 0; v < V; ++v) h[i][v] += res.value(v);
       }
     }
-    finish_row<T, V, E, false>(p, row, threads, t, h, s, [&] {
+    finish_row<T, V, E, false, false>(p, row, threads, t, h, s, [&] {
       const int64_t next = row + static_cast<int64_t>(slots) * gridDim.x;
       if (t == 0 && next < p.rows) {
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -431,6 +501,88 @@ __global__ void __launch_bounds__(512, 2) k_norm_quantize_ring(const __grid_cons
         if (mbar_try_wait(smem_u32(&bars[i]), 0) || mbar_try_wait(smem_u32(&bars[i]), 1)) break;
     atomicOr(p.error_word, 1u);
   }
+}
+
+// Rows of any alignment and length: the same ring, filled by 4-byte asynchronous copies of the aligned words that hold a
+// row; a thread shifts its vector out of them. `area` bytes of a slot hold a row's words.
+template <typename T, int V, int E>
+__global__ void __launch_bounds__(512, 2) k_norm_quantize_any(const __grid_constant__ NormArgs p, int slots, int area) {
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ Shared s;
+  const int threads = blockDim.x, t = threadIdx.x, dim = static_cast<int>(p.dim);
+  const int slot_bytes = area * (p.residual != nullptr ? 2 : 1), row_bytes = dim * static_cast<int>(sizeof(T));
+  const Span span_x = span_of(p.x, p.rows, p.x_stride * static_cast<int64_t>(sizeof(T)), row_bytes);
+  const Span span_r = span_of(p.residual, p.rows, p.residual_stride * static_cast<int64_t>(sizeof(T)), row_bytes);
+  auto bring = [&](const T* from, const Span& span, uint8_t* to) {
+    const uintptr_t first = reinterpret_cast<uintptr_t>(from) & ~static_cast<uintptr_t>(3);
+    const int words = static_cast<int>((reinterpret_cast<uintptr_t>(from) + row_bytes - first + 3) / 4);
+    for (int i = t; i < words; i += threads) {
+      const uintptr_t a = first + 4 * static_cast<uintptr_t>(i);
+      if (a >= span.lo && a + 4 <= span.hi) {
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(to) + 4 * i), "l"(a) : "memory");
+      } else {  // a word that reaches beyond the matrix, at its two ends
+#pragma unroll
+        for (int b = 0; b < 4; b += 2)
+          if (a + b >= span.lo && a + b + 2 <= span.hi)
+            *reinterpret_cast<uint16_t*>(to + 4 * i + b) = *reinterpret_cast<const uint16_t*>(a + b);
+      }
+    }
+  };
+  auto fetch = [&](int64_t row, int slot) {
+    if (row < p.rows) {
+      bring(static_cast<const T*>(p.x) + row * p.x_stride, span_x, ring + slot * slot_bytes);
+      if (p.residual != nullptr)
+        bring(static_cast<const T*>(p.residual) + row * p.residual_stride, span_r, ring + slot * slot_bytes + area);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  auto take = [&](const T* from, const uint8_t* words, int j) {  // the vector at element j
+    Piece<T, V> v;
+    const uint4 a = *reinterpret_cast<const uint4*>(words + j * sizeof(T));
+    v.w[0] = a.x, v.w[1] = a.y, v.w[2] = a.z, v.w[3] = a.w;
+    if (sizeof(T) == 2 && (reinterpret_cast<uintptr_t>(from) & 2) != 0) {
+      const uint32_t next = *reinterpret_cast<const uint32_t*>(words + j * sizeof(T) + 16);
+      v.w[0] = __funnelshift_r(a.x, a.y, 16), v.w[1] = __funnelshift_r(a.y, a.z, 16);
+      v.w[2] = __funnelshift_r(a.z, a.w, 16), v.w[3] = __funnelshift_r(a.w, next, 16);
+    }
+    return v;
+  };
+  for (int i = 0; i + 1 < slots; ++i) fetch(blockIdx.x + static_cast<int64_t>(i) * gridDim.x, i);
+  int slot = 0;
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    if (slots == 2) asm volatile("cp.async.wait_group 0;" ::: "memory");
+    else if (slots == 3) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else asm volatile("cp.async.wait_group 2;" ::: "memory");
+    __syncthreads();  // this row is here, and the slot of the row before it has been read by every thread
+    fetch(row + static_cast<int64_t>(slots - 1) * gridDim.x, slot == 0 ? slots - 1 : slot - 1);
+    const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
+    const T* r = static_cast<const T*>(p.residual) + row * p.residual_stride;
+    const uint8_t* words = ring + slot * slot_bytes;
+    float h[E][V];
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const int j = (i * threads + t) * V;
+      Piece<T, V> in;
+      in.clear();
+      if (j < dim) in = take(x, words, j);
+#pragma unroll
+      for (int v = 0; v < V; ++v) h[i][v] = j + v < dim ? in.value(v) : 0.0f;
+    }
+    if (p.residual != nullptr) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const int j = (i * threads + t) * V;
+        Piece<T, V> in;
+        in.clear();
+        if (j < dim) in = take(r, words + area, j);
+#pragma unroll
+        for (int v = 0; v < V; ++v) h[i][v] += j + v < dim ? in.value(v) : 0.0f;
+      }
+    }
+    finish_row<T, V, E, false, true>(p, row, threads, t, h, s, [] {});
+    if (++slot == slots) slot = 0;
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 unsigned int grid_of(int64_t ctas) { return static_cast<unsigned int>(ctas < (1 << 30) ? ctas : (1 << 30)); }
@@ -478,6 +630,24 @@ bool launch_ring(const NormArgs& a, const DeviceInfo& dev, int least_per_sm, cud
   return true;
 }
 
+template <typename T, int V, int E>
+bool launch_any(const NormArgs& a, const DeviceInfo& dev, cudaStream_t stream) {
+  const int64_t vecs = (a.dim + V - 1) / V;
+  const int threads = static_cast<int>(((vecs + E - 1) / E + 31) / 32 * 32);
+  if (threads > 512) return false;
+  const int64_t area = (a.dim * static_cast<int64_t>(sizeof(T)) + 15) / 16 * 16 + 32;  // a word more, vectors read whole
+  const int64_t slot_bytes = area * (a.residual != nullptr ? 2 : 1);
+  int64_t per_sm = 1024 / threads;
+  if (per_sm > kRingBytes / (2 * slot_bytes)) per_sm = kRingBytes / (2 * slot_bytes);
+  if (per_sm < 1) return false;
+  int64_t slots = kRingBytes / per_sm / slot_bytes;
+  if (slots > 4) slots = 4;
+  const int64_t ctas = static_cast<int64_t>(dev.sms) * per_sm;
+  k_norm_quantize_any<T, V, E><<<static_cast<unsigned int>(a.rows < ctas ? a.rows : ctas), threads, slots * slot_bytes, stream>>>(
+      a, static_cast<int>(slots), static_cast<int>(area));
+  return true;
+}
+
 template <typename T>
 imd_status_t launch(NormArgs a, cudaStream_t stream) {
   const DeviceInfo* dev = device_info();
@@ -496,6 +666,8 @@ imd_status_t launch(NormArgs a, cudaStream_t stream) {
   if (vec && a.dim / V > 64 &&
       (launch_ring<T, V, 4>(a, *dev, 4, stream) || launch_ring<T, V, 2>(a, *dev, 2, stream) || launch_ring<T, V, 4>(a, *dev, 1, stream)))
     return cudaGetLastError() == cudaSuccess ? IMD_STATUS_SUCCESS : IMD_STATUS_CUDA_ERROR;
+  if (!vec && a.dim >= 256 && (launch_any<T, V, 2>(a, *dev, stream) || launch_any<T, V, 4>(a, *dev, stream)))
+    return cudaGetLastError() == cudaSuccess ? IMD_STATUS_SUCCESS : IMD_STATUS_CUDA_ERROR;
   if (!(vec ? launch_registers<T, V>(a, stream) : launch_registers<T, 1>(a, stream)))
     k_norm_quantize_long<T><<<grid_of(a.rows), 1024, 0, stream>>>(a);
   return cudaGetLastError() == cudaSuccess ? IMD_STATUS_SUCCESS : IMD_STATUS_CUDA_ERROR;
@@ -510,7 +682,10 @@ bool norm_setup() {
   };
   return smem(k_norm_quantize_ring<float, 4, 2>) && smem(k_norm_quantize_ring<float, 4, 4>) &&
          smem(k_norm_quantize_ring<__half, 8, 2>) && smem(k_norm_quantize_ring<__half, 8, 4>) &&
-         smem(k_norm_quantize_ring<__nv_bfloat16, 8, 2>) && smem(k_norm_quantize_ring<__nv_bfloat16, 8, 4>);
+         smem(k_norm_quantize_ring<__nv_bfloat16, 8, 2>) && smem(k_norm_quantize_ring<__nv_bfloat16, 8, 4>) &&
+         smem(k_norm_quantize_any<float, 4, 2>) && smem(k_norm_quantize_any<float, 4, 4>) &&
+         smem(k_norm_quantize_any<__half, 8, 2>) && smem(k_norm_quantize_any<__half, 8, 4>) &&
+         smem(k_norm_quantize_any<__nv_bfloat16, 8, 2>) && smem(k_norm_quantize_any<__nv_bfloat16, 8, 4>);
 }
 
 imd_status_t norm_quantize_launch(const NormArgs& a, cudaStream_t stream) {

@@ -146,7 +146,7 @@ def test_norm_range(dim, to):
     assert torch.isnan(s[1:]).all()
 
 
-@pytest.mark.parametrize("t, dim", [(BF16, 520), (F16, 1024), (F32, 1028), (BF16, 4096), (F32, 4100), (BF16, 8200), (F16, 16384), (F32, 8192), (BF16, 20480)])
+@pytest.mark.parametrize("t, dim", [(BF16, 520), (F16, 1024), (F32, 1028), (BF16, 4096), (F32, 4100), (BF16, 8200), (F16, 16384), (F32, 8192), (BF16, 20480), (BF16, 5001), (F32, 1025), (F16, 579)])
 def test_norm_rows_in_a_ring(t, dim):
     """Many rows (those that leave the range among them), with and without a residual, in place, broadcast."""
     rows = 5003
