@@ -444,8 +444,8 @@ bool dense4_setup() {
 // 1001 26 against 24 us, 1000 x 4000 x 1001 218 against 109 us.
 constexpr int64_t kLeastWork = INT64_C(1) << 28;
 bool dense4_takes(const LinearArgs& a) {
-  return a.kind == WeightKind::kU4 && a.k > 0 && a.rows > 16 &&
-         (rows_for_tma(a.x, a.rows, 2 * a.x_stride, 2 * a.k) || a.rows * a.n * a.k >= kLeastWork);
+  return a.kind == WeightKind::kU4 && a.k > 0 && a.rows > 16 && a.rows <= kMostRowsTma && a.n <= kMostRowsTma &&
+         (rows_for_tma(a.x, a.rows, 2 * a.x_stride, 2 * a.k) || a.rows * a.n >= kLeastWork / a.k);
 }
 
 imd_status_t dense4_launch(const LinearArgs& a, cudaStream_t stream) {

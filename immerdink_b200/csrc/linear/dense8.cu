@@ -618,10 +618,10 @@ bool dense8_setup() { return set_attributes<true>() && set_attributes<false>(); 
 
 // The tensor-core kernels take rows of any alignment; with little work those are quicker in the small kernel (int8,
 // 1000 x 300 x 777: 12 against 28 us; 100 x 5000 x 4001: 74 against 54 us, 2000 x 5000 x 4001: 958 against 299 us).
-constexpr int64_t kLeastWork = INT64_C(1) << 30;
+constexpr int64_t kLeastWork = INT64_C(1) << 30, kMostRowsAny = 65535 * 256;  // (a grid's third extent)
 bool dense8_takes(const LinearArgs& a) {
   if (a.kind == WeightKind::kU4 || a.k == 0) return false;
-  return (a.rows > 16 && a.rows * a.n * a.k >= kLeastWork) || (rows_for_tma(a.x, a.rows, a.x_stride, a.k) && rows_for_tma(a.w, a.n, a.w_stride, a.k));
+  return (a.rows > 16 && a.rows <= kMostRowsAny && a.n <= kMostRowsTma && a.rows * a.n >= kLeastWork / a.k) || (rows_for_tma(a.x, a.rows, a.x_stride, a.k) && rows_for_tma(a.w, a.n, a.w_stride, a.k));
 }
 
 imd_status_t dense8_launch(const LinearArgs& a, cudaStream_t stream) {

@@ -6,6 +6,9 @@ aligns (2^-23 of the partial sum, at most A), an ordinary addition rounds (2^-24
 of the accumulations (one per instruction of at least 16 terms, partial sums no larger than the result's spread) add up to no
 more than max(sqrt(m), m / 16) 2^-23 of the result."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -376,6 +379,48 @@ def test_linear_w4_strides_and_special_values(rows):
     assert int(empty.count_nonzero()) == 0
 
 
+@pytest.mark.parametrize("k", [1, 2, 130, 255, 257, 1000, 2051])
+def test_padded_rows_of_odd_length(k):
+    """Rows in whole 16-byte units whose last unit is only partly theirs: what lies behind a row's end is a NaN or any
+    nibble and is not seen."""
+    n, group, pitch = 70, 32, -(-k // 32) * 32
+    for rows in (1, 2, 16, 20, 40, 300):
+        x, w, scale, z = operands4(BF16, rows, n, k, group, True, rows)
+        bx = torch.full((rows, pitch), math.nan, dtype=BF16, device="cuda")
+        bw = torch.full((n, pitch // 2), 255, dtype=torch.uint8, device="cuda")
+        bx[:, :k], bw[:, :(k + 1) // 2] = x, w
+        if k % 2:
+            bw[:, k // 2] |= 0xF0
+        out, intact = guarded(rows, n, F32, pad=3)
+        imd.linear_w4(bx[:, :k], bw[:, :(k + 1) // 2], out, scale, zeros=z, group=group)
+        check_product(out, *want4(x, w, scale, z, group), k)
+        assert intact()
+        for kind in (I8, E4M3):
+            x, w, xs, ws = operands8(kind, rows, n, k, rows)
+            bx = torch.full((rows, pitch), 0x7F, dtype=torch.uint8, device="cuda").view(kind)
+            bw = torch.full((n, pitch), 0x7F, dtype=torch.uint8, device="cuda").view(kind)
+            bx[:, :k], bw[:, :k] = x, w
+            imd.scaled_linear(bx[:, :k], bw[:, :k], out, xs, ws)
+            check_product(out, *want8(x, w, xs, ws), k)
+            assert intact()
+
+
+@pytest.mark.parametrize("rows, n, k", [(130, 1100, 8191), (40, 3001, 9001), (700, 901, 2047)])
+def test_unaligned_rows_with_much_work(rows, n, k):
+    """Odd row lengths on the tensor-core kernels: no row starts at a unit of anything."""
+    for kind in (I8, E4M3):
+        x, w, xs, ws = operands8(kind, rows, n, k, 7)
+        out, intact = guarded(rows, n, F32, pad=1)
+        imd.scaled_linear(x, w, out, xs, ws)
+        check_product(out, *want8(x, w, xs, ws), k)
+        assert intact()
+    for t, group in ((BF16, 128), (F16, 32)):
+        x, w, scale, z = operands4(t, rows, n, k, group, True, 8)
+        imd.linear_w4(x, w, out, scale, zeros=z, group=group)
+        check_product(out, *want4(x, w, scale, z, group), k)
+        assert intact()
+
+
 # ---- together ------------------------------------------------------------------------------------------------------
 
 class Layer:
@@ -458,6 +503,31 @@ def test_layer_captured(rows):
     graphs[0][0].replay()
     torch.cuda.synchronize()
     a.check()
+
+
+FIRST_CALL = """
+import torch, immerdink_b200 as imd
+x = torch.randn(40, 256, device="cuda").bfloat16()
+w = torch.randint(0, 256, (300, 128), device="cuda", dtype=torch.uint8)
+s = torch.rand(300, 2, device="cuda").bfloat16()
+y = torch.zeros(40, 300, device="cuda", dtype=torch.bfloat16)
+torch.cuda.synchronize()
+g, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+with torch.cuda.graph(g, stream=stream):
+    imd.linear_w4(x, w, y, s, stream=stream)
+g.replay()
+torch.cuda.synchronize()
+z = torch.empty_like(y)
+imd.linear_w4(x, w, z, s)
+torch.cuda.synchronize()
+assert torch.equal(y, z) and int(y.count_nonzero()) > 0
+"""
+
+
+def test_first_call_in_a_capture():
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
 
 
 def test_two_streams_at_once():
