@@ -48,6 +48,7 @@ struct Params {
   int32_t tiles_t, cols, stages;  // row tiles of x; rows of x per tile, padded to 16
   int32_t acc_cols;               // tensor-memory columns of one accumulator, a power of two
   int32_t wide;                   // rows of w are 16-byte aligned: they come by TMA
+  int32_t scale_quad;             // 16-bit scales whose rows are whole 16-byte units
   int32_t out_wide;               // four neighbours of the output are aligned
   unsigned int* error_word;
 };
@@ -115,6 +116,30 @@ __device__ __forceinline__ void finish_tile(const Params& p, uint32_t sums, int6
         }
       }
   }
+}
+
+// Scales of a row from group i on, as bits: eight 16-bit ones in a 16-byte load (quad) or up to four, one per word. Lanes hold
+// different rows, so a load costs 32 lookups whatever its width, and one per group took 270 cycles of the load unit a group
+// (1 x 8 warps). Predicated, so that no branch's end waits for the loads.
+__device__ __forceinline__ void load_scales(const void* scales, bool quad, bool wide, int64_t i, int left, uint32_t (&v)[4]) {
+  const uint8_t* at = static_cast<const uint8_t*>(scales) + (i << (wide ? 2 : 1));
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = 0;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %5, 0;\n\t@p ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+      : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3])
+      : "l"(at), "r"(quad && left > 0 ? 1u : 0u));
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    asm volatile(
+        "{\n\t.reg .pred a, b;\n\tsetp.ne.u32 a, %2, 0;\n\tsetp.ne.u32 b, %3, 0;\n\t@a ld.global.nc.u32 %0, [%1];\n\t"
+        "@b ld.global.nc.u16 %0, [%1];\n\t}"
+        : "+r"(v[j])
+        : "l"(at + (j << (wide ? 2 : 1))), "r"(!quad && wide && j < left ? 1u : 0u), "r"(!quad && !wide && j < left ? 1u : 0u));
+}
+__device__ __forceinline__ float scale_value(int32_t type, uint32_t bits) {
+  if (type == IMD_TYPE_F32) return __uint_as_float(bits);
+  return type == IMD_TYPE_BF16 ? __uint_as_float(bits << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
 }
 
 template <typename X, int GROUP, bool ANY>
@@ -352,15 +377,14 @@ k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUte
     int acc = 0;
     uint32_t acc_phase = 0;
     const int g1 = u1 * kGroups;
-    auto scale_of = [&](int g) {
-      return g < groups ? load_scale(p.a.scale4, p.a.scale_type, nc * p.a.scale_stride + g) : 0.0f;
-    };
-    // four groups' scales are loaded four groups ahead. The loop over the groups stays rolled: the roles' hot
+    // four or eight groups' scales are loaded as many groups ahead. The loop over the groups stays rolled: the roles' hot
     // loops together have to fit the instruction cache (unrolled by four: 400 against 376 us at 2048 x 8192 x 8192)
     const int g0 = u0 * kGroups;
-    float scale[4], next[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) next[i] = scale_of(g0 + i);
+    const bool scale_wide = p.a.scale_type == IMD_TYPE_F32, quad = p.scale_quad && g0 % 8 == 0;
+    const int ahead = quad ? 8 : 4;
+    uint32_t scale[4], next[4];
+    auto fetch_scales = [&](int g) { load_scales(p.a.scale4, quad, scale_wide, nc * p.a.scale_stride + g, groups - g, next); };
+    fetch_scales(g0);
     // ANY: rows of x that TMA cannot bring. These warps bring them, as far ahead as the ring allows: a stage is free
     // once the group that used it is complete.
     const int blocks = (u1 - u0) * kBlocks;
@@ -388,15 +412,16 @@ k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUte
     if (ANY) bring(p.stages);
 #pragma unroll 1
     for (int g = g0; g < g1; ++g) {
-      const int i = (g - g0) & 3;
+      const int i = (g - g0) & (ahead - 1);
       if (i == 0) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          scale[j] = next[j];
-          next[j] = scale_of(g + 4 + j);
-        }
+        for (int j = 0; j < 4; ++j) scale[j] = next[j];
+        fetch_scales(g + ahead);
       }
-      const float s = i == 0 ? scale[0] : i == 1 ? scale[1] : i == 2 ? scale[2] : scale[3];
+      const int word = quad ? i >> 1 : i;
+      uint32_t bits = word == 0 ? scale[0] : word == 1 ? scale[1] : word == 2 ? scale[2] : scale[3];
+      if (quad) bits = i & 1 ? bits >> 16 : bits & 0xFFFFu;
+      const float s = scale_value(p.a.scale_type, bits);
       if (!mbar_wait(tfull(acc), acc_phase, abort)) break;
       tc_fence_after();
 #pragma unroll
@@ -488,6 +513,9 @@ imd_status_t dense4_launch(const LinearArgs& a, cudaStream_t stream) {
   p.acc_cols = 32;
   while (p.acc_cols < p.cols) p.acc_cols *= 2;
   p.wide = rows_for_tma(a.w, a.n, a.w_stride, (a.k + 1) / 2);
+  const int64_t groups = (a.k + a.group - 1) / a.group;
+  p.scale_quad = a.scale_type != IMD_TYPE_F32 && groups % 8 == 0 && reinterpret_cast<uintptr_t>(a.scale4) % 16 == 0 &&
+                 (a.n == 1 || a.scale_stride % 8 == 0);
   const int size = a.out_type == IMD_TYPE_F32 ? 4 : 2;
   p.out_wide = reinterpret_cast<uintptr_t>(a.out) % (4 * size) == 0 && (a.rows == 1 || a.out_stride % 4 == 0);
   p.error_word = dev->error_word;
