@@ -31,7 +31,7 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kRegsLaunch = 128;                                   // 65536 / kThreads
-constexpr int kRegsIssue = 40, kRegsUnpack = 88, kRegsSum = 192;  // per thread of warpgroup 0, 1, 2 and 3
+constexpr int kRegsIssue = 56, kRegsUnpack = 56, kRegsSum = 200;  // per thread of warpgroup 0, 1, 2 and 3
 static_assert(kRegsIssue + kRegsUnpack + 2 * kRegsSum <= 4 * kRegsLaunch, "register shares above the launch's total");
 constexpr int kTileM = 128, kTileN = 256;
 constexpr int kBlockK = 64;                                        // k of one pipeline stage: 128 bytes a row
