@@ -15,8 +15,11 @@
 //         (rows that TMA cannot bring: x by warpgroups 2 and 3, each row's weights by the thread that unpacks it)
 //   1     thread r turns row r of the weights' next 64 k into 16-bit floats in the swizzled layout
 //   2, 3  halves of the rows of x: out += scale * accumulator, then the stores
-// Bound by shared memory traffic for many rows (the operand tiles are written and read at about the port's rate),
-// by the unpacking's issue rate for few. A cluster of up to 8 CTAs splits K (whole groups) where the row tiles
+// Bound by what the roles' own loops take at one to three warps per scheduler: 1000 to 1150 cycles a block of 64 k with
+// groups of 128 (the MMAs of 256 rows of x need 512; a second unpacking warpgroup changes nothing), 500 more for
+// each further group in it. 28672 x 8192, g128: 140 us at 33 rows, 155 at 256; 2048 x 8192 x 8192 304 us (0.55 of the measured
+// bf16 rate), with groups of 64 440, of 32 758. Hence few and wide instructions a group: multiply-adds in pairs (316 against 304
+// us), eight scales in one load. A cluster of up to 8 CTAs splits K (whole groups) where the row tiles
 // alone would not fill the GPU; the parts are added through distributed shared memory in rank order.
 // Every wait is bounded, as in the 8-bit kernels.
 #include <cstdint>
@@ -31,6 +34,7 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kRegsLaunch = 128;                                   // 65536 / kThreads
+// (56, 56, 200: no role spills; less for warpgroup 0 did)
 constexpr int kRegsIssue = 56, kRegsUnpack = 56, kRegsSum = 200;  // per thread of warpgroup 0, 1, 2 and 3
 static_assert(kRegsIssue + kRegsUnpack + 2 * kRegsSum <= 4 * kRegsLaunch, "register shares above the launch's total");
 constexpr int kTileM = 128, kTileN = 256;
@@ -119,8 +123,8 @@ __device__ __forceinline__ void finish_tile(const Params& p, uint32_t sums, int6
 }
 
 // Scales of a row from group i on, as bits: eight 16-bit ones in a 16-byte load (quad) or up to four, one per word. Lanes hold
-// different rows, so a load costs 32 lookups whatever its width, and one per group took 270 cycles of the load unit a group
-// (1 x 8 warps). Predicated, so that no branch's end waits for the loads.
+// different rows, so a load costs 32 lookups whatever its width: one load per group and warp took 270 cycles of the load unit
+// a group (33 rows x 28672 x 8192, g64: 190 against 164 us). Predicated, so that no branch's end waits for the loads.
 __device__ __forceinline__ void load_scales(const void* scales, bool quad, bool wide, int64_t i, int left, uint32_t (&v)[4]) {
   const uint8_t* at = static_cast<const uint8_t*>(scales) + (i << (wide ? 2 : 1));
 #pragma unroll
@@ -314,7 +318,7 @@ k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUte
     fetch_zeros(kb0);
     if (!p.wide) fetch_row(kb0, 0);
     // Rolled, as are the other roles' loops: one warp of each scheduler runs this code, so what does not fit the
-    // smallest instruction cache is fetched again at every turn (unrolled over a block: 1400 cycles a block).
+    // smallest instruction cache is fetched again at every turn.
 #pragma unroll 1
     for (int kb = kb0; kb < kb1; ++kb) {
       const int b = (kb - kb0) % kChunkBlocks, c = (kb - kb0) / kChunkBlocks;
@@ -371,14 +375,14 @@ k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUte
     const int c0 = wg == 2 ? 0 : half, width = wg == 2 ? half : max(p.cols - half, 0);
     const int groups = static_cast<int>((p.a.k + GROUP - 1) / GROUP);
     const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + c0;
-    float sum[128];
+    uint64_t sum[64];  // pairs
 #pragma unroll
-    for (int j = 0; j < 128; ++j) sum[j] = 0.0f;
+    for (int j = 0; j < 64; ++j) sum[j] = 0;
     int acc = 0;
     uint32_t acc_phase = 0;
     const int g1 = u1 * kGroups;
     // four or eight groups' scales are loaded as many groups ahead. The loop over the groups stays rolled: the roles' hot
-    // loops together have to fit the instruction cache (unrolled by four: 400 against 376 us at 2048 x 8192 x 8192)
+    // loops share a small instruction cache (unrolled by four it was slower by 6 % at 2048 x 8192 x 8192)
     const int g0 = u0 * kGroups;
     const bool scale_wide = p.a.scale_type == IMD_TYPE_F32, quad = p.scale_quad && g0 % 8 == 0;
     const int ahead = quad ? 8 : 4;
@@ -430,7 +434,10 @@ k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUte
           uint32_t v[32];
           tmem_load_32(taddr + acc * p.acc_cols + c, v);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) sum[c + j] = fmaf(s, __uint_as_float(v[j]), sum[c + j]);
+          for (int j = 0; j < 32; j += 2)
+            asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %3};\n\tfma.rn.f32x2 %0, a, b, %0;\n\t}"
+                : "+l"(sum[(c + j) / 2])
+                : "r"(v[j]), "r"(v[j + 1]), "r"(__float_as_uint(s)));
         }
       }
       tc_fence_before();
@@ -445,7 +452,9 @@ k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUte
 #pragma unroll
     for (int j = 0; j < 128; ++j)
       if (j < width)
-        asm volatile("st.shared.f32 [%0], %1;" ::"r"(tiles + ((c0 + j) * kTileM + row) * 4), "f"(sum[j]) : "memory");
+        asm volatile("st.shared.u32 [%0], %1;" ::"r"(tiles + ((c0 + j) * kTileM + row) * 4),
+                     "r"(static_cast<uint32_t>(sum[j / 2] >> (32 * (j & 1))))
+                     : "memory");
     __syncwarp();
   }
 
@@ -493,8 +502,8 @@ bool dense4_setup() {
   return true;
 }
 
-// Rows of any alignment with little work are quicker in the small kernel: 1802 x 83 x 150 9 against 27 us; 100 x 4000 x
-// 1001 26 against 24 us, 1000 x 4000 x 1001 218 against 109 us.
+// Rows of any alignment with little work are quicker in the small kernel (1802 x 83 x 150 9.6 against 20 us, 50 x 1000 x 1001
+// 7.9 against 11.9), with more here (100 x 4000 x 1001 26 against 18 us, 1000 x 4000 x 1001 218 against 99).
 constexpr int64_t kLeastWork = INT64_C(1) << 28;
 bool dense4_takes(const LinearArgs& a) {
   return a.kind == WeightKind::kU4 && a.k > 0 && a.rows > 16 && a.rows <= kMostRowsTma && a.n <= kMostRowsTma &&

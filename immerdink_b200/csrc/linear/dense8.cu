@@ -2,7 +2,8 @@
 //
 //   out[t, n] = xs[t] ws[n] sum_k x[t, k] w[n, k]         int8: exact int32 sums; e4m3: 32-bit float sums
 //
-// Bound by the tensor pipe once both operands have a few hundred rows, by the weights' bytes below.
+// Bound by the tensor pipe once both operands have a few hundred rows (int8 8192^3 333 us, 3300 T/s), by the weights'
+// bytes below (e4m3 48 x 28672 x 8192 42 us, 5.7 TB/s, 0.87 of the measured copy rate; 1 row 41 us).
 // Two kernels share the pipeline of the contraction's GEMM (TMA into a ring of 128-byte K blocks with the
 // 128-byte swizzle, one thread issuing tcgen05.mma, accumulators in tensor memory):
 //

@@ -3,7 +3,8 @@
 //   h = x + r;  y_j = h_j * rsqrt(mean h^2 + eps) * w_j;  a = max_j |y_j|;  scale = a / Q;
 //   q_j = round(y_j * (Q / a))                                       Q = 127 (int8), 448 (e4m3)
 //
-// Bound by HBM: 2 + 2 + 2 + 1 bytes per element for 16-bit x with a residual that is written back.
+// Bound by HBM: 2 + 2 + 2 + 1 bytes per element for 16-bit x with a residual that is written back (8191 x 8192: 78 us, 6.0
+// TB/s, 0.92 of the measured copy rate; f32 135 us, 0.99). Without a residual and for int8 bound by issue.
 // A row is read once: its values stay in registers (`E` vectors per thread) through both row
 // reductions, the sum of squares and the largest |y|. Short rows take one warp each, longer rows
 // one CTA; rows beyond the register capacity are read three times (twice from L2).
@@ -432,7 +433,8 @@ k_norm_quantize(const __grid_constant__ NormArgs p) {
 
 // Many rows: a persistent CTA whose rows arrive by bulk copies in a ring of shared memory, so that the bytes
 // in flight do not depend on registers and the next rows arrive while this one is reduced and stored. A slot
-// is refilled right after the row's first reduction, whose barrier says that every thread has read it.
+// is refilled right after the row's first reduction, whose barrier says that every thread has read it. (8191 x 8192 bf16
+// with the residual 78 us, rows loaded to registers 108.)
 template <typename T, int V, int E>
 __global__ void __launch_bounds__(512, 2) k_norm_quantize_ring(const __grid_constant__ NormArgs p, int slots) {
   extern __shared__ __align__(16) uint8_t ring[];
@@ -508,7 +510,7 @@ __global__ void __launch_bounds__(512, 2) k_norm_quantize_ring(const __grid_cons
 }
 
 // Rows of any alignment and length: the same ring, filled by 4-byte asynchronous copies of the aligned words that hold a
-// row; a thread shifts its vector out of them. `area` bytes of a slot hold a row's words.
+// row; a thread shifts its vector out of them (4096 x 5001 bf16 70 us, element by element 155). `area` bytes of a slot hold a row's words.
 template <typename T, int V, int E>
 __global__ void __launch_bounds__(512, 2) k_norm_quantize_any(const __grid_constant__ NormArgs p, int slots, int area) {
   extern __shared__ __align__(16) uint8_t ring[];

@@ -2,8 +2,9 @@
 //
 //   out[t, n] = sum_g ws[n, g] sum_{k in g} x[t, k] (w[n, k] - z[n, g])
 //
-// Bound by HBM (n k / 2 bytes) and, next to it, by the issue of the unpacking (about 12 instructions for 8 weights
-// and lane). A persistent CTA walks tiles of 16 MT rows of w; its eight warps take 256 k of every row (a piece) in
+// Bound by the issue and latency of the unpacking (18.7 instructions for 8 weights and lane, 11 of them the unpacking itself)
+// at 16 warps per SM, well before HBM (n k / 2 bytes): 1 row x 28672 x 8192 34 us with groups of 128 (3.6 TB/s, 0.55 of the
+// measured copy rate), 44 us with groups of 64 and zero points; 16 rows 60 and 67 us. A persistent CTA walks tiles of 16 MT rows of w; its eight warps take 256 k of every row (a piece) in
 // turn. A warp has its own ring of pieces that arrive by TMA, one instruction each, so the bytes in flight depend
 // on neither registers nor occupancy and a warp waits for nobody within a tile; at the end of a tile the
 // warps' sums are folded in a fixed order. x, scales and zero points of the next piece are loaded to registers
@@ -352,8 +353,9 @@ bool stream_setup() {
   return ok;
 }
 
-// Up to 16 rows in one pass over the weights; up to 32 in two, which still beats the tensor-core kernel's unpacking (17
-// rows x 28672 x 8192, g64: 130 against 180 us).
+// Up to 16 rows in one pass over the weights; up to 32 in two, which beats the tensor-core kernel where the weights are
+// many (x 28672 x 8192, g64 with zero points: 17 rows 112 against 157 us, 32 rows 134 against 157) and costs little where
+// they are few (x 4096 x 4096, g128: 17 rows 15.9 against 16.0 us, 32 rows 20.7 against 16.3).
 constexpr int64_t kPassRows = 16, kMostRows = 32;
 
 bool stream_takes(const LinearArgs& a) {
