@@ -98,6 +98,24 @@ def test_norm_sizes(rows, dim, t, to):
     norm_check(x, None, w, q2, s2, None, 0.0, t)
 
 
+@pytest.mark.parametrize("rows", [2, 600])
+@pytest.mark.parametrize("dim", [8196, 12001, 14128, 16384, 16385])
+def test_norm_long_rows_of_32_bits(rows, dim):
+    x, r, w = rnd(1, rows, dim), rnd(2, rows, dim, scale=3.0), 1 + 0.3 * rnd(3, dim)
+    h, intact = guarded(rows, dim, F32, pad=(-dim) % 4 + 4)
+    for to in (I8, E4M3):
+        q, scale = torch.empty(rows, dim, dtype=to, device="cuda"), torch.empty(rows, device="cuda")
+        imd.norm_quantize(x, w, q, scale, eps=1e-5, residual=r, residual_out=h)
+        norm_check(x, r, w, q, scale, h, 1e-5, F32)
+        assert intact()
+        imd.norm_quantize(x, w, q, scale)
+        norm_check(x, None, w, q, scale, None, 1e-6, F32)
+    q2, s2 = torch.empty_like(q), torch.empty_like(scale)
+    imd.norm_quantize(x, w, q, scale, residual=r)
+    imd.norm_quantize(x, w, q2, s2, residual=r, residual_out=x)        # in place
+    assert torch.equal(x, h) and torch.equal(q2.view(I8), q.view(I8)) and torch.equal(s2, scale)
+
+
 @pytest.mark.parametrize("t, dim", [(BF16, 640), (F16, 4096), (F32, 2052), (BF16, 33000)])
 def test_norm_strides_alignment_and_in_place(t, dim):
     rows = 5
@@ -377,6 +395,33 @@ def test_linear_w4_strides_and_special_values(rows):
     empty = torch.full((rows, n), 7.0, dtype=BF16, device="cuda")
     imd.linear_w4(x[:, :0], w[:, :0], empty, scale[:, :0], group=group)
     assert int(empty.count_nonzero()) == 0
+
+
+@pytest.mark.parametrize("t", [BF16, F16])
+@pytest.mark.parametrize("n, k, group", [(130, 2048, 128), (300, 4096, 64), (129, 1792, 32), (700, 1152, 128), (19000, 1024, 128)])
+def test_linear_w4_layouts_give_the_same(n, k, group, t):
+    """Scales and outputs at other addresses, row distances and types: the values of the call that reads and writes whole units."""
+    groups = k // group
+    for rows in (3, 17, 40, 128, 200, 300) if n < 10000 else (40,):
+        x, w, scale, z = operands4(t, rows, n, k, group, True, rows)
+        out = torch.empty(rows, n, device="cuda")
+        imd.linear_w4(x, w, out, scale, zeros=z, group=group)
+        check_product(out, *want4(x, w, scale, z, group), k)
+        for start, pad in [(1, 0), (0, 1), (0, 8), (8, 8), (3, 5)]:
+            base = torch.full((n * (groups + pad) + start + 16,), math.nan, dtype=t, device="cuda")
+            moved = base[start:start + n * (groups + pad)].view(n, groups + pad)[:, :groups]
+            moved.copy_(scale)
+            got = torch.empty_like(out)
+            imd.linear_w4(x, w, got, moved, zeros=z, group=group)
+            assert torch.equal(got, out), (rows, start, pad)
+        got = torch.empty_like(out)
+        imd.linear_w4(x, w, got, scale.float(), zeros=z, group=group)   # (another order of the sums is allowed)
+        check_product(got, *want4(x, w, scale, z, group), k)
+        for dtype in (F32, t):
+            for skew, pad in [(0, -n % 8 + 8), (1, 3), (2, -n % 4 + 4), (0, -n % 2 + 1)]:
+                got, intact = guarded(rows, n, dtype, pad=pad, skew=skew)
+                imd.linear_w4(x, w, got, scale, zeros=z, group=group)
+                assert torch.equal(got, out.to(dtype)) and intact(), (rows, dtype, skew, pad)
 
 
 @pytest.mark.parametrize("k", [1, 2, 130, 255, 257, 1000, 2051])
