@@ -17,7 +17,8 @@ const DeviceInfo* device_info();
 // Rows that TMA can bring: 16-byte units, not overlapping, few enough for 32-bit coordinates of whole tiles.
 constexpr int64_t kMostRowsTma = INT64_C(1) << 30;
 inline bool rows_for_tma(const void* p, int64_t rows, int64_t stride_bytes, int64_t row_bytes) {
-  return rows <= kMostRowsTma && reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows == 1 || (stride_bytes % 16 == 0 && stride_bytes >= row_bytes));
+  return rows <= kMostRowsTma && reinterpret_cast<uintptr_t>(p) % 16 == 0 &&
+         (rows == 1 || (stride_bytes % 16 == 0 && stride_bytes >= row_bytes));
 }
 // Tensor map of such rows as bytes, boxes of box_rows x 128 bytes with the 128-byte swizzle; what lies outside is zero.
 bool encode_rows_128(const DeviceInfo& dev, CUtensorMap* map, const void* base, int64_t row_bytes, int64_t rows,

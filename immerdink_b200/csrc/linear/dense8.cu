@@ -622,7 +622,8 @@ bool dense8_setup() { return set_attributes<true>() && set_attributes<false>(); 
 constexpr int64_t kLeastWork = INT64_C(1) << 30, kMostRowsAny = 65535 * 256;  // (a grid's third extent)
 bool dense8_takes(const LinearArgs& a) {
   if (a.kind == WeightKind::kU4 || a.k == 0) return false;
-  return (a.rows > 16 && a.rows <= kMostRowsAny && a.n <= kMostRowsTma && a.rows * a.n >= kLeastWork / a.k) || (rows_for_tma(a.x, a.rows, a.x_stride, a.k) && rows_for_tma(a.w, a.n, a.w_stride, a.k));
+  return (a.rows > 16 && a.rows <= kMostRowsAny && a.n <= kMostRowsTma && a.rows * a.n >= kLeastWork / a.k) ||
+         (rows_for_tma(a.x, a.rows, a.x_stride, a.k) && rows_for_tma(a.w, a.n, a.w_stride, a.k));
 }
 
 imd_status_t dense8_launch(const LinearArgs& a, cudaStream_t stream) {

@@ -672,9 +672,11 @@ imd_status_t launch(NormArgs a, cudaStream_t stream) {
   if (vec && a.dim / V > 64 &&
       (launch_ring<T, V, 4>(a, *dev, 4, stream) || launch_ring<T, V, 2>(a, *dev, 2, stream) || launch_ring<T, V, 4>(a, *dev, 1, stream)))
     return cudaGetLastError() == cudaSuccess ? IMD_STATUS_SUCCESS : IMD_STATUS_CUDA_ERROR;
-  // (f32 rows of 12001 to 16384: with the residual two of them fill the ring, and repeated passes are quicker: 75 against 91 us at
+  // (f32 rows of 8193 to 16384 elements with a residual: two slots fill the ring, registers are quicker, 76 against 91 us at
   // 1000 x 12001; without it 42 against 63)
-  if (!vec && a.dim >= 256 && (launch_any<T, V, 2>(a, *dev, stream) || launch_any<T, V, 4>(a, *dev, stream) || (a.residual == nullptr && launch_any<T, V, 32 / V>(a, *dev, stream))))
+  if (!vec && a.dim >= 256 &&
+      (launch_any<T, V, 2>(a, *dev, stream) || launch_any<T, V, 4>(a, *dev, stream) ||
+       (a.residual == nullptr && launch_any<T, V, 32 / V>(a, *dev, stream))))
     return cudaGetLastError() == cudaSuccess ? IMD_STATUS_SUCCESS : IMD_STATUS_CUDA_ERROR;
   if (!(vec ? launch_registers<T, V>(a, stream) : launch_registers<T, 1>(a, stream)))
     k_norm_quantize_long<T><<<grid_of(a.rows), 1024, 0, stream>>>(a);

@@ -4,11 +4,12 @@
 //
 // Bound by the issue and latency of the unpacking (18.7 instructions for 8 weights and lane, 11 of them the unpacking itself)
 // at 16 warps per SM, well before HBM (n k / 2 bytes): 1 row x 28672 x 8192 34 us with groups of 128 (3.6 TB/s, 0.55 of the
-// measured copy rate), 44 us with groups of 64 and zero points; 16 rows 60 and 67 us. A persistent CTA walks tiles of 16 MT rows of w; its eight warps take 256 k of every row (a piece) in
-// turn. A warp has its own ring of pieces that arrive by TMA, one instruction each, so the bytes in flight depend
-// on neither registers nor occupancy and a warp waits for nobody within a tile; at the end of a tile the
-// warps' sums are folded in a fixed order. x, scales and zero points of the next piece are loaded to registers
-// under the products of this one.
+// measured copy rate), 44 us with groups of 64 and zero points; 16 rows 60 and 67 us.
+//
+// A persistent CTA walks tiles of 16 MT rows of w; its eight warps take 256 k of every row (a piece) in turn. A warp has its
+// own ring of pieces that arrive by TMA, one instruction each, so the bytes in flight depend on neither registers nor
+// occupancy and a warp waits for nobody within a tile; at the end of a tile the warps' sums are folded in a fixed order. x,
+// scales and zero points of the next piece are loaded to registers under the products of this one.
 //
 // Products are mma.sync of 16 rows of w by 8 rows of x. The order of k inside an instruction is free as long as
 // both operands use the same one: a lane takes consecutive k of its quarter of a group with one load, and the words
