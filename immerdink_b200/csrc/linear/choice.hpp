@@ -1,0 +1,51 @@
+// Which kernel takes a product: the rules on sizes, types and alignment, apart from the kernels so that a host
+// program can ask them (tests/linear_choice_shim.cpp).
+#pragma once
+#include <cstdint>
+
+#include "linear.hpp"
+
+namespace imd {
+
+// Rows that TMA can bring: 16-byte units, not overlapping. Its coordinates are 32-bit: few enough rows for whole tiles, and
+// rows short enough for whole blocks of k (which start at most 256 bytes behind a row's end) counted in bytes.
+constexpr int64_t kMostRowsTma = INT64_C(1) << 30, kMostBytesTma = (INT64_C(1) << 31) - 512;
+inline bool rows_for_tma(const void* p, int64_t rows, int64_t stride_bytes, int64_t row_bytes) {
+  return rows <= kMostRowsTma && row_bytes <= kMostBytesTma && reinterpret_cast<uintptr_t>(p) % 16 == 0 &&
+         (rows == 1 || (stride_bytes % 16 == 0 && stride_bytes >= row_bytes));
+}
+inline bool x4_for_tma(const LinearArgs& a) { return rows_for_tma(a.x, a.rows, 2 * a.x_stride, 2 * a.k); }
+inline bool w4_for_tma(const LinearArgs& a) { return rows_for_tma(a.w, a.n, a.w_stride, (a.k + 1) / 2); }
+inline bool both8_for_tma(const LinearArgs& a) {
+  return rows_for_tma(a.x, a.rows, a.x_stride, a.k) && rows_for_tma(a.w, a.n, a.w_stride, a.k);
+}
+
+// 8 bits: the tensor-core kernels take rows of any alignment; with little work those are quicker in the small kernel (int8,
+// 1000 x 300 x 777: 12 against 28 us; 100 x 5000 x 4001: 74 against 54 us, 2000 x 5000 x 4001: 958 against 299 us).
+constexpr int64_t kLeastWork8 = INT64_C(1) << 30, kMostRowsAny8 = 65535 * 256;  // (a grid's third extent)
+inline bool dense8_takes(const LinearArgs& a) {
+  if (a.kind == WeightKind::kU4 || a.k == 0) return false;
+  return (a.rows > 16 && a.rows <= kMostRowsAny8 && a.n <= kMostRowsTma && a.rows * a.n >= kLeastWork8 / a.k) ||
+         both8_for_tma(a);
+}
+
+// 4 bits, streamed. Up to 16 rows in one pass over the weights; up to 32 in two, which beats the tensor-core kernel where
+// the weights are many (x 28672 x 8192, g64 with zero points: 17 rows 112 against 157 us, 32 rows 134 against 157) and costs
+// little where they are few (x 4096 x 4096, g128: 17 rows 15.9 against 16.0 us, 32 rows 20.7 against 16.3).
+// The kernel walks k in 32 bits, up to eight pieces of 256 and a step past a row's end.
+constexpr int64_t kStreamPassRows = 16, kStreamMostRows = 32, kStreamMostK = (INT64_C(1) << 31) - 4096;
+inline bool stream_takes(const LinearArgs& a) {
+  return a.kind == WeightKind::kU4 && a.rows <= kStreamMostRows && a.k > 0 && a.k <= kStreamMostK &&
+         reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && (a.rows == 1 || a.x_stride % 8 == 0) && w4_for_tma(a);
+}
+
+// 4 bits on the tensor cores. Rows of any alignment with little work are quicker in the small kernel (1802 x 83 x 150 9.6
+// against 20 us, 50 x 1000 x 1001 7.9 against 11.9), with more here (100 x 4000 x 1001 26 against 18 us, 1000 x 4000 x 1001 218
+// against 99).
+constexpr int64_t kLeastWork4 = INT64_C(1) << 28;
+inline bool dense4_takes(const LinearArgs& a) {
+  return a.kind == WeightKind::kU4 && a.k > 0 && a.rows > 16 && a.rows <= kMostRowsTma && a.n <= kMostRowsTma &&
+         (x4_for_tma(a) || a.rows * a.n >= kLeastWork4 / a.k);
+}
+
+}  // namespace imd

@@ -445,7 +445,7 @@ k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUte
       if (lane == 0) mbar_arrive(tempty(acc));
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1u;
-      if (ANY) bring((g + 1 - g0) * GROUP / kBlockK + p.stages);
+      if (ANY) bring((g + 1 - g0) / kGroups * kBlocks + p.stages);
     }
     __syncwarp();
     // the ring is free: the last group's accumulator was complete, so every operand had been read
@@ -502,14 +502,6 @@ bool dense4_setup() {
   return true;
 }
 
-// Rows of any alignment with little work are quicker in the small kernel (1802 x 83 x 150 9.6 against 20 us, 50 x 1000 x 1001
-// 7.9 against 11.9), with more here (100 x 4000 x 1001 26 against 18 us, 1000 x 4000 x 1001 218 against 99).
-constexpr int64_t kLeastWork = INT64_C(1) << 28;
-bool dense4_takes(const LinearArgs& a) {
-  return a.kind == WeightKind::kU4 && a.k > 0 && a.rows > 16 && a.rows <= kMostRowsTma && a.n <= kMostRowsTma &&
-         (rows_for_tma(a.x, a.rows, 2 * a.x_stride, 2 * a.k) || a.rows * a.n >= kLeastWork / a.k);
-}
-
 imd_status_t dense4_launch(const LinearArgs& a, cudaStream_t stream) {
   const DeviceInfo* dev = device_info();
   if (dev == nullptr) return IMD_STATUS_CUDA_ERROR;
@@ -521,7 +513,7 @@ imd_status_t dense4_launch(const LinearArgs& a, cudaStream_t stream) {
   p.cols = a.rows < kTileN ? static_cast<int32_t>((a.rows + 15) / 16 * 16) : kTileN;
   p.acc_cols = 32;
   while (p.acc_cols < p.cols) p.acc_cols *= 2;
-  p.wide = rows_for_tma(a.w, a.n, a.w_stride, (a.k + 1) / 2);
+  p.wide = w4_for_tma(a);
   const int64_t groups = (a.k + a.group - 1) / a.group;
   p.scale_quad = a.scale_type != IMD_TYPE_F32 && groups % 8 == 0 && reinterpret_cast<uintptr_t>(a.scale4) % 16 == 0 &&
                  (a.n == 1 || a.scale_stride % 8 == 0);
@@ -533,7 +525,7 @@ imd_status_t dense4_launch(const LinearArgs& a, cudaStream_t stream) {
   if (p.stages > kMaxStages) p.stages = kMaxStages;
 
   // the swizzle goes by bytes, so x is described as bytes too
-  const bool any = !rows_for_tma(a.x, a.rows, 2 * a.x_stride, 2 * a.k);
+  const bool any = !x4_for_tma(a);
   CUtensorMap map_x{}, map_w{};
   if ((!any && !encode_rows_128(*dev, &map_x, a.x, 2 * a.k, a.rows, 2 * a.x_stride, p.cols)) ||
       (p.wide && !encode_rows_128(*dev, &map_w, a.w, (a.k + 1) / 2, a.n, a.w_stride, kTileM)))

@@ -602,8 +602,7 @@ bool set_attributes() {
 
 template <bool I8>
 bool launch(const LinearArgs& a, const DeviceInfo& dev, const Params& p, cudaStream_t stream) {
-  if (!rows_for_tma(a.x, a.rows, a.x_stride, a.k) || !rows_for_tma(a.w, a.n, a.w_stride, a.k))
-    return launch_swap<I8, true>(a, dev, p, stream);
+  if (!both8_for_tma(a)) return launch_swap<I8, true>(a, dev, p, stream);
   if (a.rows <= 256) return launch_swap<I8, false>(a, dev, p, stream);
   // whole waves of tiles on the CTA pairs: 128 columns where their last wave is fuller by more than the
   // narrower tile costs
@@ -616,15 +615,6 @@ bool launch(const LinearArgs& a, const DeviceInfo& dev, const Params& p, cudaStr
 }  // namespace
 
 bool dense8_setup() { return set_attributes<true>() && set_attributes<false>(); }
-
-// The tensor-core kernels take rows of any alignment; with little work those are quicker in the small kernel (int8,
-// 1000 x 300 x 777: 12 against 28 us; 100 x 5000 x 4001: 74 against 54 us, 2000 x 5000 x 4001: 958 against 299 us).
-constexpr int64_t kLeastWork = INT64_C(1) << 30, kMostRowsAny = 65535 * 256;  // (a grid's third extent)
-bool dense8_takes(const LinearArgs& a) {
-  if (a.kind == WeightKind::kU4 || a.k == 0) return false;
-  return (a.rows > 16 && a.rows <= kMostRowsAny && a.n <= kMostRowsTma && a.rows * a.n >= kLeastWork / a.k) ||
-         (rows_for_tma(a.x, a.rows, a.x_stride, a.k) && rows_for_tma(a.w, a.n, a.w_stride, a.k));
-}
 
 imd_status_t dense8_launch(const LinearArgs& a, cudaStream_t stream) {
   const DeviceInfo* dev = device_info();

@@ -354,20 +354,10 @@ bool stream_setup() {
   return ok;
 }
 
-// Up to 16 rows in one pass over the weights; up to 32 in two, which beats the tensor-core kernel where the weights are
-// many (x 28672 x 8192, g64 with zero points: 17 rows 112 against 157 us, 32 rows 134 against 157) and costs little where
-// they are few (x 4096 x 4096, g128: 17 rows 15.9 against 16.0 us, 32 rows 20.7 against 16.3).
-constexpr int64_t kPassRows = 16, kMostRows = 32;
-
-bool stream_takes(const LinearArgs& a) {
-  return a.kind == WeightKind::kU4 && a.rows <= kMostRows && a.k > 0 && reinterpret_cast<uintptr_t>(a.x) % 16 == 0 &&
-         (a.rows == 1 || a.x_stride % 8 == 0) && rows_for_tma(a.w, a.n, a.w_stride, (a.k + 1) / 2);
-}
-
 imd_status_t stream_launch(const LinearArgs& all, cudaStream_t stream) {
   const DeviceInfo* dev = device_info();
   if (dev == nullptr) return IMD_STATUS_CUDA_ERROR;
-  const int64_t passes = (all.rows + kPassRows - 1) / kPassRows, share = (all.rows + passes - 1) / passes;
+  const int64_t passes = (all.rows + kStreamPassRows - 1) / kStreamPassRows, share = (all.rows + passes - 1) / passes;
   for (int64_t t0 = 0; t0 < all.rows; t0 += share) {
     LinearArgs a = all;
     a.rows = all.rows - t0 < share ? all.rows - t0 : share;

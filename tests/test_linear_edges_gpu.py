@@ -1,0 +1,37 @@
+"""Calls at the edges of what the quantised linear layer accepts, on a GPU, against plain 64-bit arithmetic."""
+import pytest
+import torch
+
+import immerdink_b200 as imd
+from immerdink_b200 import linear
+
+pytestmark = pytest.mark.gpu
+BF16, F16, F32, I8, E4M3 = torch.bfloat16, torch.float16, torch.float32, torch.int8, torch.float8_e4m3fn
+
+
+@pytest.fixture(autouse=True)
+def no_wait_gave_up():
+    yield
+    assert linear.load_library().device_error() == 0
+
+
+@pytest.mark.parametrize("rows, k, skew, gib", [(17, (1 << 30) + 64, 1, 44), (1, (1 << 31) - 1, 0, 8)])
+def test_linear_w4_depth_beyond_30_bits(rows, k, skew, gib):
+    """Sums whose terms lie at both ends of a row and around 2^29, 2^30 and 2^31: x is zero elsewhere, so a sum has as many
+    terms as places; each term and addition rounds once (2^-24), or is cut (2^-23) in a tensor instruction."""
+    if torch.cuda.mem_get_info()[0] < gib << 30:
+        pytest.skip("not enough free memory")
+    places = [p for p in (0, 777, (1 << 29) - 1, 1 << 29, (1 << 30) - 1, 1 << 30, (1 << 31) - 300, k - 130, k - 1) if p < k]
+    x = torch.zeros(rows, k, dtype=BF16, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(5)
+    values = torch.randn(rows, len(places), generator=g, device="cuda").to(BF16)
+    x[:, places] = values
+    half, groups = (k + 1) // 2, -(-k // 128)
+    w = torch.randint(0, 256, (half + skew,), generator=g, device="cuda", dtype=torch.uint8)[skew:].view(1, half)
+    scale = (0.5 + torch.rand(1, groups, generator=g, device="cuda")).to(BF16)
+    out = torch.empty(rows, 1, device="cuda")
+    imd.linear_w4(x, w, out, scale)
+    nibble = torch.stack([(w[0, p // 2] >> (4 * (p & 1))) & 15 for p in places]).double() - 8
+    terms = values.double() * nibble * torch.stack([scale[0, p // 128] for p in places]).double()
+    assert bool(((out[:, 0].double() - terms.sum(1)).abs() <= 2 * len(places) * 2.0 ** -23 * terms.abs().sum(1)).all())
+    assert bool((terms[:, len(places) // 2:].abs().sum(1) > 0.01 * terms.abs().sum(1)).all())   # what a short walk would lose
