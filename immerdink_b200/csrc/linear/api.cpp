@@ -52,6 +52,7 @@ imd_status_t imd_norm_quantize(int64_t rows, int64_t dim, int32_t x_type, const 
     return IMD_STATUS_INVALID_VALUE;
   if (weight_type != x_type && weight_type != IMD_TYPE_F32) return IMD_STATUS_NOT_SUPPORTED;
   if (rows == 0) return IMD_STATUS_SUCCESS;
+  if (rows == 1) x_stride = residual_stride = residual_out_stride = q_stride = dim;  // a single row has no distance
   if (x == nullptr || weight == nullptr || q == nullptr || scale == nullptr ||
       (residual_out != nullptr && residual == nullptr) || !in_stride_ok(x_stride) ||
       (residual != nullptr && !in_stride_ok(residual_stride)) ||
@@ -93,6 +94,8 @@ imd_status_t imd_scaled_linear(int64_t rows, int64_t n, int64_t k, int32_t type,
     return IMD_STATUS_INVALID_VALUE;
   if (type == IMD_TYPE_I8 && k > kMaxI8Depth) return IMD_STATUS_NOT_SUPPORTED;
   if (rows == 0 || n == 0) return IMD_STATUS_SUCCESS;
+  if (rows == 1) x_stride = k, out_stride = n;
+  if (n == 1) w_stride = k;
   if ((k > 0 && (x == nullptr || w == nullptr)) || x_scale == nullptr || w_scale == nullptr ||
       out == nullptr || !in_stride_ok(x_stride) || !in_stride_ok(w_stride) ||
       !out_stride_ok(out_stride, rows, n))
@@ -126,6 +129,8 @@ imd_status_t imd_linear_w4(int64_t rows, int64_t n, int64_t k, int32_t group, in
     return IMD_STATUS_NOT_SUPPORTED;
   if (rows == 0 || n == 0) return IMD_STATUS_SUCCESS;
   const int64_t groups = (k + group - 1) / group, half = (k + 1) / 2;
+  if (rows == 1) x_stride = k, out_stride = n;
+  if (n == 1) w_stride = half, scale_stride = zeros_stride = groups;
   if ((k > 0 && (x == nullptr || w == nullptr || w_scale == nullptr)) || out == nullptr ||
       !in_stride_ok(x_stride) || !in_stride_ok(w_stride) || !in_stride_ok(scale_stride) ||
       (zeros != nullptr && !in_stride_ok(zeros_stride)) || !out_stride_ok(out_stride, rows, n))

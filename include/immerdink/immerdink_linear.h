@@ -15,8 +15,8 @@
  * its checks touches nothing. Results do not depend on the run: no atomics, sums in a fixed order.
  *
  * Matrices are row-major with unit stride inside a row; `*_stride` is the distance between rows in
- * ELEMENTS of the matrix (bytes for packed 4-bit weights). Inputs may repeat rows (stride 0);
- * an output's rows must not overlap. Every buffer is aligned to its element size; any alignment
+ * ELEMENTS of the matrix (bytes for packed 4-bit weights), not looked at for a single row. Inputs may
+ * repeat rows (stride 0); an output's rows must not overlap. Every buffer is aligned to its element size; any alignment
  * above that is optional (16-byte aligned rows take the wide loads).
  *
  * Checks, in order: types and sizes out of range -> INVALID_VALUE (a combination that exists in no

@@ -35,3 +35,26 @@ def test_linear_w4_depth_beyond_30_bits(rows, k, skew, gib):
     terms = values.double() * nibble * torch.stack([scale[0, p // 128] for p in places]).double()
     assert bool(((out[:, 0].double() - terms.sum(1)).abs() <= 2 * len(places) * 2.0 ** -23 * terms.abs().sum(1)).all())
     assert bool((terms[:, len(places) // 2:].abs().sum(1) > 0.01 * terms.abs().sum(1)).all())   # what a short walk would lose
+
+
+@pytest.mark.parametrize("t", [BF16, F32])
+def test_one_row_in_place_whatever_its_stride(t):
+    """The last position of a sequence: buf[:, -1] and its view(1, dim) are the same row with different strides."""
+    dim = 264
+    buf, w = torch.randn(1, 5, dim, device="cuda").to(t), torch.randn(dim, device="cuda").to(t)
+    x, same = buf[:, -1], buf[:, -1].view(1, dim)
+    assert x.stride(0) != same.stride(0) and x.data_ptr() == same.data_ptr()
+    r = torch.randn(1, dim, device="cuda").to(t)
+    q, s, h = torch.empty(1, dim, dtype=I8, device="cuda"), torch.empty(1, device="cuda"), torch.empty(1, dim, dtype=t, device="cuda")
+    imd.norm_quantize(x.clone(), w, q, s, residual=r, residual_out=h)
+    before = buf.clone()
+    for out, target in ((same, "x"), (x, "x"), (same, "residual"), (x, "residual")):
+        buf.copy_(before)
+        q2, s2 = torch.empty_like(q), torch.empty_like(s)
+        first = x if out is same else same
+        if target == "x":
+            imd.norm_quantize(first, w, q2, s2, residual=r, residual_out=out)
+        else:
+            imd.norm_quantize(r, w, q2, s2, residual=first, residual_out=out)
+        assert torch.equal(same, h) and torch.equal(q2, q) and torch.equal(s2, s)
+        assert torch.equal(buf[:, :-1], before[:, :-1])
