@@ -114,7 +114,7 @@ def build_cuda(force=False, verbose=False):
 
 def build_linear(force=False, verbose=False):
     """libimmerdink_linear.so stands alone: it shares headers with the others but needs neither."""
-    src_time = _newest([os.path.join(CSRC, "linear"), os.path.join(CSRC, "cuda"), INCLUDE])
+    src_time = _newest([os.path.join(CSRC, "linear"), os.path.join(CSRC, "cuda"), os.path.join(CSRC, "common"), INCLUDE])
     if not force and os.path.exists(LINEAR_LIB) and os.path.getmtime(LINEAR_LIB) >= src_time:
         return LINEAR_LIB
     os.makedirs(OBJ_DIR, exist_ok=True)

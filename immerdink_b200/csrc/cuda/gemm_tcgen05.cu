@@ -162,7 +162,7 @@ k_gemm_i8(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     if (lane == 0) {
       int stage = 0;
       uint32_t phase = 0;
-      uint32_t issued = 0;  // bit s: a load into stage s is (or was) in flight
+      uint32_t issued = 0;
       bool okay = true;
       const uint64_t pol_a = l2_policy(p.l2_hints & 3), pol_b = l2_policy((p.l2_hints >> 2) & 3);
       for (int64_t w = blockIdx.x; w < total && okay; w += gridDim.x) {
@@ -177,20 +177,14 @@ k_gemm_i8(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           const int kx = p.s.k0 + kb * kTileK;
           tma_load_3d(dst, &map_a, full(stage), kx, c.tm * kTileM, c.plane, pol_a);
           tma_load_3d(dst + kBytesA, &map_b, full(stage), kx, c.tn * kTileN, c.plane, pol_b);
-          issued |= 1u << stage;
+          ++issued;
           if (++stage == kStages) {
             stage = 0;
             phase ^= 1u;
           }
         }
       }
-      if (!okay) {
-        // give the copies still in flight a bounded time to land before the CTA exits
-        for (int s = 0; s < kStages; ++s)
-          if (issued & (1u << s))
-            for (uint32_t it = 0; it < (1u << 20); ++it)
-              if (mbar_try_wait(full(s), 0) || mbar_try_wait(full(s), 1)) break;
-      }
+      let_land(issued, kStages, full);
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
@@ -386,7 +380,7 @@ k_gemm_i8_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     if (lane == 0) {
       int stage = 0;
       uint32_t phase = 0;
-      uint32_t issued = 0;  // bit s: a load into stage s is (or was) in flight
+      uint32_t issued = 0;
       bool okay = true;
       const uint64_t pol_a = l2_policy(p.l2_hints & 3), pol_b = l2_policy((p.l2_hints >> 2) & 3);
       for (int64_t w = first; w < total && okay; w += step) {
@@ -405,21 +399,14 @@ k_gemm_i8_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                            c.plane, pol_a);
           tma_load_3d_pair(dst + kBytesA, &map_b, leader_full, kx,
                            c.tn * 256 + static_cast<int>(rank) * 128, c.plane, pol_b);
-          issued |= 1u << stage;
+          ++issued;
           if (++stage == kPairStages) {
             stage = 0;
             phase ^= 1u;
           }
         }
       }
-      if (!okay && leader) {
-        // give the copies of both CTAs still in flight a bounded time to land (they complete on
-        // the leader's barriers) before the pair passes its final cluster barrier and exits
-        for (int s = 0; s < kPairStages; ++s)
-          if (issued & (1u << s))
-            for (uint32_t it = 0; it < (1u << 20); ++it)
-              if (mbar_try_wait(full(s), 0) || mbar_try_wait(full(s), 1)) break;
-      }
+      let_land_pair(leader, !okay, issued, kPairStages, full);  // then the pair's last cluster barrier
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer (leader CTA only) ----------------

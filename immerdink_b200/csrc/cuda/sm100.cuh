@@ -5,9 +5,12 @@
 
 #include <cuda.h>
 
+#include "common/ring.hpp"
+
 namespace imd {
 
 constexpr uint32_t kSpinLimit = 1u << 26;  // try_wait polls before a wait gives up
+constexpr uint32_t kLandLimit = 1u << 20;  // and before copies in flight are given up
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
@@ -43,6 +46,25 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
   }
   *abort = 1;
   return false;
+}
+
+// Waits, with a limit, until the copies of a ring's first `issued` loads have landed; full(s): the barrier of slot s. Who
+// loads ends with it, whether all is loaded or a wait gave up, so that no copy arrives in memory that is given back.
+template <typename Full>
+__device__ __forceinline__ void let_land(uint32_t issued, int slots, Full full) {
+  await_ring(issued, slots, kLandLimit, [&](int s, uint32_t parity) { return mbar_try_wait(full(s), parity); });
+}
+// The same where nobody knows how many loads there were when a wait gave up: of every slot (at most 32).
+template <typename Full>
+__device__ __forceinline__ void let_land_any(int slots, Full full) {
+  await_slots(slots, kLandLimit, [&](int s, uint32_t parity) { return mbar_try_wait(full(s), parity); });
+}
+// let_land in a CTA pair, where the copies of both complete on the leader's barriers. After a wait that gave up, one of the
+// peer's for a stage that the leader had not armed shows nowhere: the peer waits for a fixed time, about a millisecond.
+template <typename Full>
+__device__ __forceinline__ void let_land_pair(bool leader, bool gave_up, uint32_t issued, int slots, Full full) {
+  if (leader) let_land(issued, slots, full);
+  else if (gave_up) for (int i = 0; i < 1024; ++i) __nanosleep(1000);
 }
 
 // L2 eviction policy of an operand load.

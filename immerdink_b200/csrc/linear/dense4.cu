@@ -206,26 +206,18 @@ k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUte
     if (!ANY && warp == 0 && lane == 0) {
       int stage = 0;
       uint32_t phase = 0, issued = 0;
-      bool okay = true;
       const uint64_t policy = l2_policy(1);  // x is read by every row tile of the weights
       for (int kb = u0 * kBlocks; kb < u1 * kBlocks; ++kb) {
-        if (!mbar_wait(empty(stage), phase ^ 1u, abort)) {
-          okay = false;
-          break;
-        }
+        if (!mbar_wait(empty(stage), phase ^ 1u, abort)) break;
         mbar_expect_tx(full(stage), p.cols * 128);
         tma_load_3d(tiles + stage * stage_bytes + kBytesM, &map_x, full(stage), kb * 2 * kBlockK, static_cast<int>(t0), 0, policy);
-        issued |= 1u << stage;
+        ++issued;
         if (++stage == p.stages) {
           stage = 0;
           phase ^= 1u;
         }
       }
-      if (!okay)  // copies still in flight get a bounded time to land
-        for (int s = 0; s < p.stages; ++s)
-          if (issued & (1u << s))
-            for (uint32_t it = 0; it < (1u << 20); ++it)
-              if (mbar_try_wait(full(s), 0) || mbar_try_wait(full(s), 1)) break;
+      let_land(issued, p.stages, full);
     } else if (warp == 1 && lane == 0) {
       constexpr uint32_t kType = std::is_same<X, __nv_bfloat16>::value ? 1u : 0u;
       const uint32_t idesc = (1u << 4) | (kType << 7) | (kType << 10) | (static_cast<uint32_t>(p.cols >> 3) << 17) |
@@ -275,10 +267,7 @@ k_dense4(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUte
         tma_load_3d(packed + slot * kChunkBytes, &map_w, wfull(slot), (u0 * kBlocks + c * kChunkBlocks) * (kBlockK / 2),
                     static_cast<int>(n0), 0, policy);
       }
-      if (c < chunks)  // as above: the copies of the last two chunks
-        for (int s = 0; s < 2 && s < c; ++s)
-          for (uint32_t it = 0; it < (1u << 20); ++it)
-            if (mbar_try_wait(wfull(s), 0) || mbar_try_wait(wfull(s), 1)) break;
+      let_land(c, 2, wfull);
     }
     __syncwarp();
   } else if (wg == 1) {

@@ -211,19 +211,14 @@ k_dense8_pair(const __grid_constant__ CUtensorMap map_x, const __grid_constant__
           tma_load_3d_pair(dst, &map_x, leader_full, kb * kTileK, tm * 256 + static_cast<int>(rank) * 128, 0, policy);
           tma_load_3d_pair(dst + kBytesM, &map_w, leader_full, kb * kTileK,
                            tn * BN + static_cast<int>(rank) * (BN / 2), 0, policy);
-          issued |= 1u << stage;
+          ++issued;
           if (++stage == kStages) {
             stage = 0;
             phase ^= 1u;
           }
         }
       }
-      if (!okay && leader) {  // copies still in flight get a bounded time to land before the pair ends
-        for (int s = 0; s < kStages; ++s)
-          if (issued & (1u << s))
-            for (uint32_t it = 0; it < (1u << 20); ++it)
-              if (mbar_try_wait(full(s), 0) || mbar_try_wait(full(s), 1)) break;
-      }
+      let_land_pair(leader, !okay, issued, kStages, full);  // then the pair's last cluster barrier
     }
   } else if (warp == 1) {
     if (lane == 0 && leader) {
@@ -469,29 +464,20 @@ k_dense8_swap(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
     if (lane == 0) {
       int stage = 0;
       uint32_t phase = 0, issued = 0;
-      bool okay = true;
       const uint64_t policy_w = l2_policy(2), policy_x = l2_policy(1);  // weights stream through, x stays
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait(empty(stage), phase ^ 1u, abort)) {
-          okay = false;
-          break;
-        }
+        if (!mbar_wait(empty(stage), phase ^ 1u, abort)) break;
         mbar_expect_tx(full(stage), stage_bytes);
         const uint32_t dst = tiles + stage * stage_bytes;
         tma_load_3d(dst, &map_w, full(stage), kb * kTileK, n0, 0, policy_w);
         tma_load_3d(dst + kBytesM, &map_x, full(stage), kb * kTileK, 0, 0, policy_x);
-        issued |= 1u << stage;
+        ++issued;
         if (++stage == p.stages) {
           stage = 0;
           phase ^= 1u;
         }
       }
-      if (!okay) {
-        for (int s = 0; s < p.stages; ++s)
-          if (issued & (1u << s))
-            for (uint32_t it = 0; it < (1u << 20); ++it)
-              if (mbar_try_wait(full(s), 0) || mbar_try_wait(full(s), 1)) break;
-      }
+      let_land(issued, p.stages, full);
     }
   } else if (warp == 1) {
     if (lane == 0) {

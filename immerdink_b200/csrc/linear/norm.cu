@@ -490,7 +490,7 @@ __global__ void __launch_bounds__(512, 2) k_norm_quantize_ring(const __grid_cons
     }
     finish_row<T, V, E, false, false>(p, row, threads, t, h, s, [&] {
       const int64_t next = row + static_cast<int64_t>(slots) * gridDim.x;
-      if (t == 0 && next < p.rows) {
+      if (t == 0 && next < p.rows && !*abort) {  // after a wait that gave up every barrier is passed, but nothing is fetched
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         fetch(next, slot);
       }
@@ -501,10 +501,7 @@ __global__ void __launch_bounds__(512, 2) k_norm_quantize_ring(const __grid_cons
     }
   }
   if (t == 0 && *abort) {
-    // copies still in flight get a bounded time to land before their memory is given back
-    for (int i = 0; i < slots; ++i)
-      for (uint32_t it = 0; it < (1u << 20); ++it)
-        if (mbar_try_wait(smem_u32(&bars[i]), 0) || mbar_try_wait(smem_u32(&bars[i]), 1)) break;
+    let_land_any(slots, [&](int i) { return smem_u32(&bars[i]); });
     atomicOr(p.error_word, 1u);
   }
 }

@@ -253,7 +253,8 @@ k_stream(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ Para
       Ready<C> ready;
       source.settle(raw, ready);
       source.fetch(k0 + 128, lane, raw);
-      mbar_wait(bar(slot), phase, abort);  // after a wait that gave up the values are of no use, but every barrier is passed
+      // after a wait that gave up the values are of no use and nothing more is loaded, but every barrier is passed
+      if (!mbar_wait(bar(slot), phase, abort)) load_row = tiles * kRows;
       __syncwarp();
       multiply<C>(ready, nibbles, row, 0, lane, acc);
       source.settle(raw, ready);
@@ -291,10 +292,7 @@ k_stream(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ Para
     turn ^= 1;  // the next tile's partial sums go where nobody reads any more
   }
   if (*abort && lane == 0) {
-    // copies still in flight get a bounded time to land before their memory is given back
-    for (int s = 0; s < p.slots; ++s)
-      for (uint32_t it = 0; it < (1u << 20); ++it)
-        if (mbar_try_wait(bar(s), 0) || mbar_try_wait(bar(s), 1)) break;
+    let_land_any(p.slots, bar);
     atomicOr(p.error_word, 1u);
   }
 }
