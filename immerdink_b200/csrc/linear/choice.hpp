@@ -48,4 +48,15 @@ inline bool dense4_takes(const LinearArgs& a) {
          (x4_for_tma(a) || a.rows * a.n >= kLeastWork4 / a.k);
 }
 
+// CTAs that share a tile of a tensor-core kernel by splitting K: a cluster of 1, 2, 4 or 8, as many as fit the GPU at once
+// with at least two steps of K each. A cluster lies in one part of the GPU, so 8 x 15 or 4 x 33 CTAs fit 148 SMs, not 8 x 18
+// or 4 x 37, and what does not fit costs a second round (4 bits, 40 x 2048 x 2048: clusters of 8 18.8, of 4 11.4 us; 40 x 4736 x
+// 8192: of 4 46.8, of 2 40.0; 8 bits 1 x 4736 x 8192: of 8 17.2, of 4 12.1). clusters[i]: how many of 2^i CTAs fit with one
+// CTA on an SM.
+inline int split_of(int64_t tiles, int64_t steps, const int* clusters, int ctas_per_sm) {
+  int i = 0;
+  while (i < 3 && tiles <= static_cast<int64_t>(clusters[i + 1]) * ctas_per_sm && steps >= INT64_C(4) << i) ++i;
+  return 1 << i;
+}
+
 }  // namespace imd

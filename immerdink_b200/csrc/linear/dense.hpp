@@ -10,6 +10,7 @@ struct DeviceInfo {
   void* encode_tiled = nullptr;  // cuTensorMapEncodeTiled
   unsigned int* error_word = nullptr;
   int sms = 0;
+  int clusters[4] = {};          // of 1, 2, 4 and 8 CTAs that fit at once, one CTA on an SM
 };
 // Of the current device; made on first use, nullptr where that fails (asked again at the next call).
 const DeviceInfo* device_info();
@@ -25,6 +26,7 @@ imd_status_t dense8_launch(const LinearArgs& a, cudaStream_t stream);
 bool stream_setup();
 imd_status_t stream_launch(const LinearArgs& a, cudaStream_t stream);
 bool dense4_setup();
+bool dense4_clusters(int sms, int* clusters);  // DeviceInfo's
 imd_status_t dense4_launch(const LinearArgs& a, cudaStream_t stream);
 
 }  // namespace imd

@@ -491,6 +491,22 @@ bool dense4_setup() {
   return true;
 }
 
+bool dense4_clusters(int sms, int* clusters) {  // any kernel whose shared memory leaves room for one CTA
+  for (int i = 0; i < 4; ++i) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned int>(sms), 1u << i);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kSmem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {1, 1u << i, 1};
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&clusters[i], kernel_of<__half>(128, false), &cfg) != cudaSuccess) return false;
+  }
+  return true;
+}
+
 imd_status_t dense4_launch(const LinearArgs& a, cudaStream_t stream) {
   const DeviceInfo* dev = device_info();
   if (dev == nullptr) return IMD_STATUS_CUDA_ERROR;
@@ -522,8 +538,7 @@ imd_status_t dense4_launch(const LinearArgs& a, cudaStream_t stream) {
 
   const int64_t tiles = (a.n + kTileM - 1) / kTileM * p.tiles_t;
   if (tiles >= (INT64_C(1) << 31)) return IMD_STATUS_NOT_SUPPORTED;
-  int parts = 1;  // CTAs that share a tile: enough to occupy the SMs, at least two steps of K each
-  while (parts < 8 && tiles * parts * 2 <= dev->sms && p.units >= 4 * parts) parts *= 2;
+  const int parts = split_of(tiles, p.units, dev->clusters, 1);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned int>(tiles), static_cast<unsigned int>(parts));
   cfg.blockDim = dim3(kThreads);

@@ -313,6 +313,10 @@ k_dense8_pair(const __grid_constant__ CUtensorMap map_x, const __grid_constant__
 
 // ---- up to 256 rows: weights on the M side ---------------------------------------------------------------
 constexpr int kSwapMaxStages = 12;
+// Two CTAs of an SM take turns (one stores while the other loads) as long as their rings stay deep enough (up to kSwapColsHalf
+// rows of x) and their registers allow it (checked below); bringing rows of any alignment takes more than half of them.
+template <bool ANY>
+constexpr int kSwapCtas = ANY ? 1 : 2;
 
 __device__ __forceinline__ uint32_t load_cluster(uint32_t addr) {
   uint32_t v;
@@ -518,7 +522,6 @@ k_dense8_swap(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
   }
 }
 
-// Two CTAs of an SM take turns (one stores while the other loads) as long as their rings stay deep enough.
 constexpr int kSwapSmem = 200 * 1024, kSwapSmemHalf = 110 * 1024, kSwapColsHalf = 128;
 
 template <bool I8, int BN>
@@ -555,9 +558,8 @@ bool launch_swap(const LinearArgs& a, const DeviceInfo& dev, Params p, cudaStrea
   p.x_stride = a.x_stride, p.w_stride = a.w_stride, p.k = a.k;
   const int64_t tiles = (a.n + kTileM - 1) / kTileM, tiles_z = (a.rows + p.cols - 1) / p.cols;
   if (tiles_z > 65535) return false;
-  const bool two = p.cols <= kSwapColsHalf;
-  int parts = 1;  // CTAs that share a row tile: enough to occupy the SMs, at least two K blocks each
-  while (parts < 8 && tiles * tiles_z * parts * 2 <= dev.sms * (two ? 2 : 1) && p.k_blocks >= 4 * parts) parts *= 2;
+  const bool two = kSwapCtas<ANY> == 2 && p.cols <= kSwapColsHalf;
+  const int parts = split_of(tiles * tiles_z, p.k_blocks, dev.clusters, two ? 2 : 1);
   const int stage_bytes = kBytesM + p.cols * kTileK;
   p.stages = ((two ? kSwapSmemHalf : kSwapSmem) - 1024 - kCtrlBytes) / stage_bytes;
   if (p.stages > kSwapMaxStages) p.stages = kSwapMaxStages;
@@ -580,7 +582,10 @@ bool set_attributes() {
   auto smem = [](const void* f, int bytes) {
     return cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess;
   };
-  return smem(reinterpret_cast<const void*>(k_dense8_pair<I8, 256>), kPairSmem<256>) &&
+  cudaFuncAttributes attr;
+  return cudaFuncGetAttributes(&attr, k_dense8_swap<I8, false>) == cudaSuccess &&
+         kSwapCtas<false> * kThreads * ((attr.numRegs + 7) / 8 * 8) <= 65536 &&
+         smem(reinterpret_cast<const void*>(k_dense8_pair<I8, 256>), kPairSmem<256>) &&
          smem(reinterpret_cast<const void*>(k_dense8_pair<I8, 128>), kPairSmem<128>) &&
          smem(reinterpret_cast<const void*>(k_dense8_swap<I8, false>), kSwapSmem) &&
          smem(reinterpret_cast<const void*>(k_dense8_swap<I8, true>), kSwapSmem);

@@ -22,7 +22,8 @@ bool make(int device, DeviceInfo* info) {
   if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess ||
       q != cudaDriverEntryPointSuccess || fn == nullptr || cudaGetSymbolAddress(&word, g_error_word) != cudaSuccess ||
       cudaDeviceGetAttribute(&info->sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess ||
-      !norm_setup() || !stream_setup() || !dense8_setup() || !dense4_setup())
+      !norm_setup() || !stream_setup() || !dense8_setup() || !dense4_setup() ||
+      !dense4_clusters(info->sms, info->clusters))
     return false;
   info->encode_tiled = fn;
   info->error_word = static_cast<unsigned int*>(word);

@@ -24,4 +24,8 @@ int choice_8(int e4m3, int64_t rows, int64_t n, int64_t k, int64_t x, int64_t xs
 int w4_by_tma(int64_t n, int64_t k, int64_t w, int64_t ws) {
   return imd::w4_for_tma(args(imd::WeightKind::kU4, 1, n, k, 0, 0, w, ws, 128));
 }
+int split(int64_t tiles, int64_t steps, int c1, int c2, int c4, int c8, int per_sm) {
+  const int clusters[4] = {c1, c2, c4, c8};
+  return imd::split_of(tiles, steps, clusters, per_sm);
+}
 }

@@ -22,6 +22,7 @@ def lib(tmp_path_factory):
     lib.choice_w4.argtypes = [C.c_int64] * 7 + [C.c_int]
     lib.choice_8.argtypes = [C.c_int] + [C.c_int64] * 7
     lib.w4_by_tma.argtypes = [C.c_int64] * 4
+    lib.split.argtypes = [C.c_int64, C.c_int64] + [C.c_int] * 5
     return lib
 
 
@@ -64,3 +65,17 @@ def test_rows_that_tma_brings(lib):
     assert w4(lib, 3, 64, 0) == "m" and w4(lib, 300, 64, 0) == "m"
     assert e8(lib, 3, 64, 256) == "t" and e8(lib, 3, 64, 256, w=B + 1) == "m" and e8(lib, 3, 64, 0) == "m"
     assert e8(lib, 3000, 5000, 257, ws=257) == "a" and e8(lib, 300, 50, 257, ws=257) == "m"
+
+
+def test_clusters_fit_at_once(lib):
+    """K is split among as many CTAs as the GPU holds clusters of that size at once, not as many as it has SMs."""
+    fits = (148, 74, 33, 15)
+    for per_sm in (1, 2):
+        for tiles in range(1, 400):
+            for steps in (1, 3, 4, 7, 8, 15, 16, 64):
+                parts = lib.split(tiles, steps, *fits, per_sm)
+                assert parts in (1, 2, 4, 8)
+                assert parts == 1 or (tiles <= fits[parts.bit_length() - 1] * per_sm and steps >= 2 * parts)
+                assert parts == 8 or tiles > fits[parts.bit_length()] * per_sm or steps < 4 * parts   # no less than that
+    assert [lib.split(t, 64, *fits, 1) for t in (15, 16, 33, 34, 74, 75)] == [8, 4, 4, 2, 2, 1]
+    assert [lib.split(t, 64, *fits, 2) for t in (30, 32, 37, 74, 148, 149)] == [8, 4, 4, 2, 2, 1]
