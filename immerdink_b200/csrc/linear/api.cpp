@@ -150,7 +150,9 @@ imd_status_t imd_linear_w4(int64_t rows, int64_t n, int64_t k, int32_t group, in
   a.out = out, a.out_stride = out_stride;
   a.kind = imd::WeightKind::kU4;
   a.x_type = x_type, a.scale_type = scale_type, a.out_type = out_type, a.group = group;
-  if (imd::stream_takes(a)) return imd::stream_launch(a, stream);
+  const imd::DeviceInfo* dev = imd::device_info();
+  if (dev == nullptr) return IMD_STATUS_CUDA_ERROR;
+  if (imd::stream_takes(a, dev->clusters)) return imd::stream_launch(a, stream);
   return imd::dense4_takes(a) ? imd::dense4_launch(a, stream) : imd::linear_small_launch(a, stream);
 }
 

@@ -29,13 +29,38 @@ inline bool dense8_takes(const LinearArgs& a) {
          both8_for_tma(a);
 }
 
-// 4 bits, streamed. Up to 16 rows in one pass over the weights; up to 32 in two, which beats the tensor-core kernel where
-// the weights are many (x 28672 x 8192, g64 with zero points: 17 rows 112 against 157 us, 32 rows 134 against 157) and costs
-// little where they are few (x 4096 x 4096, g128: 17 rows 15.9 against 16.0 us, 32 rows 20.7 against 16.3).
+// CTAs that share a tile of a tensor-core kernel by splitting K: a cluster of 1, 2, 4 or 8, as many as fit the GPU at once
+// with at least two steps of K each. A cluster lies in one part of the GPU, so 8 x 15 or 4 x 33 CTAs fit 148 SMs, not 8 x 18
+// or 4 x 37, and what does not fit costs a second round (4 bits, 40 x 2048 x 2048: clusters of 8 18.8, of 4 11.4 us; 40 x 4736 x
+// 8192: of 4 46.8, of 2 40.0; 8 bits 1 x 4736 x 8192: of 8 17.2, of 4 12.1). clusters[i]: how many of 2^i CTAs fit with one
+// CTA on an SM.
+inline int split_of(int64_t tiles, int64_t steps, const int* clusters, int ctas_per_sm) {
+  int i = 0;
+  while (i < 3 && tiles <= static_cast<int64_t>(clusters[i + 1]) * ctas_per_sm && steps >= INT64_C(4) << i) ++i;
+  return 1 << i;
+}
+
+// 4 bits, streamed: up to 16 rows of x in one pass over the weights. 17 to 32 take two passes where the tensor-core kernel,
+// whose time hardly depends on the rows, is slower: with groups of 32, whose sums bound it, and where its tiles leave much of
+// their last round idle; little is enough from kStreamTallN rows of w on, where a streamed tile has 32 of them.
+// (us, two passes / tensor cores, zero points: 24 x 8192 x 28672 g32 163 / 219; idle more than a third, 24 x 2048 x 2048 g128
+// 9.1 / 10.9, 24 x 4736 x 2816 g64 14 / 20; idle 14 %, 17 x 4096 x 4096 g128 16.8 / 16.1, 32 rows 20.8 / 16.4, 24 x 8192 x 8192 57
+// / 40, g64 50 / 44; many rows of w, idle a quarter, 24 x 28672 x 8192 g128 123 / 139; not idle, 24 x 18944 x 3584 g128 42 / 35.)
+// Over 18 shapes from 512 x 1024 to 128256 x 4096, 17 to 32 rows, all groups, the choice is 1.1 % slower than the better of the two
+// on average, two passes throughout 4.7 %, the tensor cores throughout 21 %; most at 32 x 512 x 16384 g128 (33 / 24).
 // The kernel walks k in 32 bits, up to eight pieces of 256 and a step past a row's end.
 constexpr int64_t kStreamPassRows = 16, kStreamMostRows = 32, kStreamMostK = (INT64_C(1) << 31) - 4096;
-inline bool stream_takes(const LinearArgs& a) {
-  return a.kind == WeightKind::kU4 && a.rows <= kStreamMostRows && a.k > 0 && a.k <= kStreamMostK &&
+constexpr int64_t kStreamTallN = 64 * 148;  // two tiles of 32 rows of w for each of 148 SMs
+inline bool two_passes(const LinearArgs& a, const int* clusters) {
+  if (a.group == 32) return true;
+  const int64_t tiles = (a.n + 127) / 128, unit = a.group > 64 ? a.group : 64;
+  const int64_t ctas = tiles * split_of(tiles, (a.k + unit - 1) / unit, clusters, 1);
+  const int64_t slots = (ctas + clusters[0] - 1) / clusters[0] * clusters[0];
+  return 100 * slots >= ctas * (a.n >= kStreamTallN ? 102 : a.group == 64 ? 136 : 150);
+}
+inline bool stream_takes(const LinearArgs& a, const int* clusters) {
+  return a.kind == WeightKind::kU4 && a.k > 0 && a.k <= kStreamMostK &&
+         (a.rows <= kStreamPassRows || (a.rows <= kStreamMostRows && two_passes(a, clusters))) &&
          reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && (a.rows == 1 || a.x_stride % 8 == 0) && w4_for_tma(a);
 }
 
@@ -46,17 +71,6 @@ constexpr int64_t kLeastWork4 = INT64_C(1) << 28;
 inline bool dense4_takes(const LinearArgs& a) {
   return a.kind == WeightKind::kU4 && a.k > 0 && a.rows > 16 && a.rows <= kMostRowsTma && a.n <= kMostRowsTma &&
          (x4_for_tma(a) || a.rows * a.n >= kLeastWork4 / a.k);
-}
-
-// CTAs that share a tile of a tensor-core kernel by splitting K: a cluster of 1, 2, 4 or 8, as many as fit the GPU at once
-// with at least two steps of K each. A cluster lies in one part of the GPU, so 8 x 15 or 4 x 33 CTAs fit 148 SMs, not 8 x 18
-// or 4 x 37, and what does not fit costs a second round (4 bits, 40 x 2048 x 2048: clusters of 8 18.8, of 4 11.4 us; 40 x 4736 x
-// 8192: of 4 46.8, of 2 40.0; 8 bits 1 x 4736 x 8192: of 8 17.2, of 4 12.1). clusters[i]: how many of 2^i CTAs fit with one
-// CTA on an SM.
-inline int split_of(int64_t tiles, int64_t steps, const int* clusters, int ctas_per_sm) {
-  int i = 0;
-  while (i < 3 && tiles <= static_cast<int64_t>(clusters[i + 1]) * ctas_per_sm && steps >= INT64_C(4) << i) ++i;
-  return 1 << i;
 }
 
 }  // namespace imd

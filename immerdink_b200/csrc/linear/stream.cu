@@ -366,7 +366,7 @@ imd_status_t stream_launch(const LinearArgs& all, cudaStream_t stream) {
     p.error_word = dev->error_word;
     p.pieces = static_cast<int32_t>((a.k + kPieceK - 1) / kPieceK);
     // 32 rows per tile share the loads of x; 16 where there would be too few tiles to occupy the SMs
-    const bool tall = a.n >= static_cast<int64_t>(32) * 2 * dev->sms;
+    const bool tall = a.n >= kStreamTallN;
     const Call c{a.x_type == IMD_TYPE_F16, a.scale_type == a.x_type, a.zeros != nullptr, tall, a.rows > 8, a.group};
     if (!choose(c, [&](auto choice) { return launch<decltype(choice)>(p, *dev, stream); })) {
       cudaGetLastError();

@@ -14,7 +14,8 @@ extern "C" {
 // 's' streamed, 't' tensor cores with x by TMA, 'a' tensor cores with x brought by loads, 'm' the small kernel
 int choice_w4(int64_t rows, int64_t n, int64_t k, int64_t x, int64_t xs, int64_t w, int64_t ws, int group) {
   const imd::LinearArgs a = args(imd::WeightKind::kU4, rows, n, k, x, xs, w, ws, group);
-  if (imd::stream_takes(a)) return 's';
+  const int clusters[4] = {148, 74, 33, 15};
+  if (imd::stream_takes(a, clusters)) return 's';
   return !imd::dense4_takes(a) ? 'm' : imd::x4_for_tma(a) ? 't' : 'a';
 }
 int choice_8(int e4m3, int64_t rows, int64_t n, int64_t k, int64_t x, int64_t xs, int64_t w, int64_t ws) {

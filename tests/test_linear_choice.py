@@ -79,3 +79,13 @@ def test_clusters_fit_at_once(lib):
                 assert parts == 8 or tiles > fits[parts.bit_length()] * per_sm or steps < 4 * parts   # no less than that
     assert [lib.split(t, 64, *fits, 1) for t in (15, 16, 33, 34, 74, 75)] == [8, 4, 4, 2, 2, 1]
     assert [lib.split(t, 64, *fits, 2) for t in (30, 32, 37, 74, 148, 149)] == [8, 4, 4, 2, 2, 1]
+
+
+@pytest.mark.parametrize("rows", [17, 24, 32])
+def test_two_streamed_passes_only_where_they_are_quicker(lib, rows):
+    for n, k in ((4096, 4096), (3584, 8192), (8192, 4096), (4096, 14336), (8192, 8192), (8192, 28672), (18944, 3584)):
+        assert w4(lib, rows, n, k) == "t" and w4(lib, rows, n, k, group=32) == "s"
+        assert w4(lib, 16, n, k) == "s" and w4(lib, 33, n, k, group=32) == "t"
+    for n, k in ((512, 1024), (1024, 4096), (2048, 2048), (4736, 2816), (14336, 4096), (28672, 8192), (128256, 4096)):
+        for group in (32, 64, 128):
+            assert w4(lib, rows, n, k, group=group) == "s"
