@@ -4,7 +4,8 @@
     libimmerdink.so        C ABI + sm_100a kernels       (nvcc -gencode arch=compute_100a,code=sm_100a)
     libimmerdink_hooks.so  the same objects + the imd_test_* / imd_prof_* entry points (tests, phase timing)
     libimmerdink_linear.so C ABI + sm_100a kernels of the quantised linear layer (nvcc)
-    _fastcall.so           its front end's host side for PyTorch tensors (g++'s C, Python.h)
+    _fastcall.<ABI>.so     its front end's host side for PyTorch tensors, for the interpreter that builds it (g++'s C,
+                           Python.h; where that is not installed calls take the way of other arrays)
 
     python -m immerdink_b200.build [--force]
 
@@ -23,7 +24,7 @@ INCLUDE = os.path.join(ROOT, "include")
 HOST_LIB = os.path.join(HERE, "libimmerdink_host.so")
 CUDA_LIB = os.path.join(HERE, "libimmerdink.so")
 HOOKS_LIB = os.path.join(HERE, "libimmerdink_hooks.so")
-FASTCALL_LIB = os.path.join(HERE, "_fastcall.so")
+FASTCALL_LIB = os.path.join(HERE, "_fastcall" + sysconfig.get_config_var("EXT_SUFFIX"))
 LINEAR_LIB = os.path.join(HERE, "libimmerdink_linear.so")
 OBJ_DIR = os.path.join(HERE, "build")
 
@@ -133,7 +134,10 @@ def build_linear(force=False, verbose=False):
 
 
 def build_fastcall(force=False):
+    """None where Python.h is not installed."""
     src = os.path.join(CSRC, "linear", "fastcall.c")
+    if not os.path.exists(os.path.join(sysconfig.get_paths()["include"], "Python.h")):
+        return None
     if force or not os.path.exists(FASTCALL_LIB) or os.path.getmtime(FASTCALL_LIB) < os.path.getmtime(src):
         _run([_cxx(), "-x", "c", "-std=gnu11", "-O2", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall",
               "-I" + sysconfig.get_paths()["include"], src, "-o", FASTCALL_LIB])
@@ -144,7 +148,8 @@ def build_all(force=False, verbose=False):
     build_host(force)
     build_cuda(force, verbose)
     build_linear(force, verbose)
-    build_fastcall(force)
+    if build_fastcall(force) is None:
+        print("no Python.h: _fastcall is left out", file=sys.stderr)
 
 
 if __name__ == "__main__":

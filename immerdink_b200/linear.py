@@ -11,9 +11,10 @@ tensors, DLPack producers or `__cuda_array_interface__` objects; bfloat16 and fl
 one of the first two. They must be on the current device, and rows must have unit stride.
 
 Calls with PyTorch tensors take a short way (csrc/linear/fastcall.c) that does the same checks in C; what
-it does not take, and everything that is refused, goes through the general path below.
+it does not take, and everything that is refused, goes through the general path below, and so does every call
+where that module was not built (a call then takes longer on the host).
 
-There is no fallback: when a library is missing, the first call raises OSError."""
+There is no CPU fallback: when the library is missing, the first call raises OSError."""
 import ctypes as C
 import os
 import threading
@@ -37,6 +38,19 @@ SIGNATURES = {
 }
 
 
+class _GeneralOnly:
+    """In the place of _fastcall where it was not built: takes no call."""
+    norm_quantize = scaled_linear = linear_w4 = learn = staticmethod(lambda *args: None)
+
+
+def _short_way():
+    try:
+        from . import _fastcall
+    except ImportError:
+        return _GeneralOnly
+    return _fastcall
+
+
 class Library:
     """libimmerdink_linear.so. Search order: `path`, $IMMERDINK_LINEAR_LIB,
     $IMMERDINK_LIB_DIR/libimmerdink_linear.so, the package directory."""
@@ -55,11 +69,7 @@ class Library:
         for name, args in SIGNATURES.items():
             f = getattr(self.lib, name)
             f.restype, f.argtypes = C.c_int, args
-        try:
-            from . import _fastcall
-        except ImportError as exc:
-            raise OSError("_fastcall.so not found (build it with `python -m immerdink_b200.build`)") from exc
-        self.fast = _fastcall
+        self.fast = _short_way()
         self._address = {name: C.cast(getattr(self.lib, name), C.c_void_p).value for name in SIGNATURES}
         self._local, self._get_device = threading.local(), None
         for name in ("libcudart.so.12", "libcudart.so.13", "libcudart.so"):
@@ -111,11 +121,6 @@ def load_library(path=None):
 _torch_types = {}   # dtype object of PyTorch -> type (None: not one of ours)
 
 
-def _learn(dtype, kind):
-    from . import _fastcall
-    _fastcall.learn(dtype, kind)
-
-
 def _view(x, what, stream, device):
     """(pointer, shape, element strides or None, type, readonly) of a CUDA array."""
     dtype = getattr(x, "dtype", None)
@@ -123,7 +128,7 @@ def _view(x, what, stream, device):
         if dtype not in _torch_types:
             _torch_types[dtype] = _TORCH_TYPES.get(str(dtype))
             if _torch_types[dtype] is not None:
-                _learn(dtype, _torch_types[dtype])
+                _short_way().learn(dtype, _torch_types[dtype])
         on = x.get_device()
         if on < 0:
             raise TypeError(f"{what} is not in CUDA memory")

@@ -58,3 +58,24 @@ def test_one_row_in_place_whatever_its_stride(t):
             imd.norm_quantize(r, w, q2, s2, residual=first, residual_out=out)
         assert torch.equal(same, h) and torch.equal(q2, q) and torch.equal(s2, s)
         assert torch.equal(buf[:, :-1], before[:, :-1])
+
+
+def test_general_way_with_tensors():
+    """Without the short way of PyTorch tensors every call does the same."""
+    lib = linear.Library()
+    lib.fast = linear._GeneralOnly
+    for rows in (1, 5):
+        x, r, w = (torch.randn(*s, device="cuda").to(BF16) for s in ((rows, 96), (rows, 96), (96,)))
+        got = []
+        for use in (None, lib):
+            q, s, h = torch.empty(rows, 96, dtype=I8, device="cuda"), torch.empty(rows, device="cuda"), torch.empty_like(x)
+            y, z = torch.empty(rows, 40, dtype=BF16, device="cuda"), torch.empty(rows, 40, dtype=BF16, device="cuda")
+            g = torch.Generator(device="cuda").manual_seed(3)
+            w8 = torch.randint(-128, 128, (40, 96), generator=g, device="cuda", dtype=torch.int32).to(I8)
+            w4 = torch.randint(0, 256, (40, 48), generator=g, device="cuda", dtype=torch.uint8)
+            scale = torch.rand(40, 3, generator=g, device="cuda").to(BF16)
+            assert imd.norm_quantize(x, w, q, s, residual=r, residual_out=h, lib=use) == (q, s)
+            assert imd.scaled_linear(q, w8, y, s, scale[:, 0].float(), lib=use) is y
+            assert imd.linear_w4(x, w4, z, scale, group=32, lib=use) is z
+            got.append((q, s, h, y, z))
+        assert all(torch.equal(a, b) for a, b in zip(*got))

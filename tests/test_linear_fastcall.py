@@ -173,3 +173,32 @@ def test_one_row_of_a_larger_array(ways):
     args = w4_args(1, 1)
     args[1] = args[1].but(_stride=(4096, 1))
     both(ways, "linear_w4", args, True)
+
+
+def test_built_for_this_interpreter(ways):
+    from immerdink_b200 import _fastcall
+    import sysconfig
+    assert _fastcall.__file__ == build.FASTCALL_LIB and build.FASTCALL_LIB.endswith(sysconfig.get_config_var("EXT_SUFFIX"))
+
+
+def test_without_the_short_way(monkeypatch, tmp_path):
+    """A machine without Python.h builds and runs everything else: calls then go the general way."""
+    monkeypatch.setattr(build, "FASTCALL_LIB", str(tmp_path / "_fastcall.so"))
+    monkeypatch.setattr(build.sysconfig, "get_paths", lambda: {"include": str(tmp_path)})
+    assert build.build_fastcall(force=True) is None and not os.path.exists(build.FASTCALL_LIB)
+    build.build_linear()
+    monkeypatch.setitem(sys.modules, "immerdink_b200._fastcall", None)
+    monkeypatch.delattr(imd, "_fastcall", raising=False)
+    lib = linear.Library()
+    a = [imd.DeviceArray(0x10000, (3, 16), None, "f2"), imd.DeviceArray(0x20000, (16,), None, "f2"), imd.DeviceArray(0x30000, (3, 16), None, "i1"),
+         imd.DeviceArray(0x40000, (3,), None, "f4")]
+    with pytest.raises(imd.InvalidValueError):
+        imd.norm_quantize(*a, eps=-1.0, lib=lib)
+    with pytest.raises(TypeError, match="CUDA memory"):
+        imd.norm_quantize(torch.zeros(2, 8, dtype=BF16), *a[1:], lib=lib)
+    with pytest.raises(imd.MisalignedError):
+        imd.norm_quantize(*a[:3], imd.DeviceArray(0x40002, (3,), None, "f4"), lib=lib)
+    with pytest.raises(imd.AliasingError):
+        imd.scaled_linear(a[2], a[2], imd.DeviceArray(0x30000, (3, 3), None, "f4"), a[3], a[3], lib=lib)
+    with pytest.raises(ValueError):
+        imd.linear_w4(a[0], a[2], a[2], a[3], group=31, lib=lib)
