@@ -18,19 +18,29 @@ bool is_float(int32_t t) { return t == IMD_TYPE_F32 || t == IMD_TYPE_BF16 || t =
 bool is_8bit(int32_t t) { return t == IMD_TYPE_I8 || t == IMD_TYPE_E4M3; }
 int size_of(int32_t t) { return t == IMD_TYPE_F32 ? 4 : is_float(t) ? 2 : 1; }
 
-// Bytes [lo, hi) of a row-major matrix; empty for a null pointer or an empty matrix.
-struct Interval {
-  i128 lo = 0, hi = 0;
+// The bytes of a row-major matrix: rows of `width`, `pitch` apart (0: one row), inside [lo, hi); empty for a null pointer or
+// an empty matrix.
+struct Bytes {
+  i128 lo = 0, hi = 0, width = 0, pitch = 0;
 };
-Interval bytes_of(const void* p, int64_t rows, int64_t cols, int64_t stride, int size) {
-  Interval r;
+Bytes bytes_of(const void* p, int64_t rows, int64_t cols, int64_t stride, int size) {
+  Bytes r;
   if (p == nullptr || rows == 0 || cols == 0) return r;
+  r.width = static_cast<i128>(cols) * size;
+  r.pitch = rows == 1 ? 0 : static_cast<i128>(stride) * size;
   r.lo = static_cast<i128>(reinterpret_cast<uintptr_t>(p));
-  r.hi = r.lo + (static_cast<i128>(rows - 1) * stride + cols) * size;
+  r.hi = r.lo + (rows - 1) * r.pitch + r.width;
   return r;
 }
-bool overlap(const Interval& x, const Interval& y) {
-  return x.lo < x.hi && y.lo < y.hi && x.lo < y.hi && y.lo < x.hi;
+// Whether two matrices may share a byte. Rows at the same distance, as columns of one buffer have, interleave without doing
+// so where one's rows begin behind the other's and end before its next; other distances are not looked into.
+bool overlap(const Bytes& x, const Bytes& y) {
+  if (x.lo >= x.hi || y.lo >= y.hi || x.lo >= y.hi || y.lo >= x.hi) return false;
+  const i128 pitch = x.pitch != 0 ? x.pitch : y.pitch;
+  if (pitch == 0 || (y.pitch != 0 && y.pitch != pitch)) return true;
+  i128 behind = (y.lo - x.lo) % pitch;
+  if (behind < 0) behind += pitch;
+  return behind < x.width || behind + y.width > pitch;
 }
 bool extent_ok(int64_t e) { return e >= 0 && e < kMaxExtent; }
 bool in_stride_ok(int64_t s) { return s >= 0 && s < (INT64_C(1) << 40); }
@@ -60,7 +70,7 @@ imd_status_t imd_norm_quantize(int64_t rows, int64_t dim, int32_t x_type, const 
       !out_stride_ok(q_stride, rows, dim))
     return IMD_STATUS_INVALID_VALUE;
   const int sx = size_of(x_type), sw = size_of(weight_type);
-  const Interval ix = bytes_of(x, rows, dim, x_stride, sx),
+  const Bytes ix = bytes_of(x, rows, dim, x_stride, sx),
                  ir = bytes_of(residual, rows, dim, residual_stride, sx),
                  iw = bytes_of(weight, 1, dim, 0, sw),
                  ih = bytes_of(residual_out, rows, dim, residual_out_stride, sx),
@@ -101,7 +111,7 @@ imd_status_t imd_scaled_linear(int64_t rows, int64_t n, int64_t k, int32_t type,
       !out_stride_ok(out_stride, rows, n))
     return IMD_STATUS_INVALID_VALUE;
   const int so = size_of(out_type);
-  const Interval io = bytes_of(out, rows, n, out_stride, so);
+  const Bytes io = bytes_of(out, rows, n, out_stride, so);
   if (overlap(io, bytes_of(x, rows, k, x_stride, 1)) || overlap(io, bytes_of(w, n, k, w_stride, 1)) ||
       overlap(io, bytes_of(x_scale, 1, rows, 0, 4)) || overlap(io, bytes_of(w_scale, 1, n, 0, 4)))
     return IMD_STATUS_ALIASING;
@@ -136,7 +146,7 @@ imd_status_t imd_linear_w4(int64_t rows, int64_t n, int64_t k, int32_t group, in
       (zeros != nullptr && !in_stride_ok(zeros_stride)) || !out_stride_ok(out_stride, rows, n))
     return IMD_STATUS_INVALID_VALUE;
   const int sx = size_of(x_type), ss = size_of(scale_type), so = size_of(out_type);
-  const Interval io = bytes_of(out, rows, n, out_stride, so);
+  const Bytes io = bytes_of(out, rows, n, out_stride, so);
   if (overlap(io, bytes_of(x, rows, k, x_stride, sx)) || overlap(io, bytes_of(w, n, half, w_stride, 1)) ||
       overlap(io, bytes_of(w_scale, n, groups, scale_stride, ss)) ||
       overlap(io, bytes_of(zeros, n, groups, zeros_stride, 1)))

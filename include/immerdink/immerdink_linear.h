@@ -21,7 +21,9 @@
  *
  * Checks, in order: types and sizes out of range -> INVALID_VALUE (a combination that exists in no
  * kernel -> NOT_SUPPORTED); an empty output -> SUCCESS; null pointers, strides -> INVALID_VALUE;
- * an output that overlaps another buffer -> ALIASING; element alignment -> MISALIGNED. */
+ * an output that overlaps another buffer -> ALIASING; element alignment -> MISALIGNED. Columns of one
+ * buffer (rows at the same distance in bytes) do not overlap where they share no byte; matrices that
+ * interleave at different distances count as overlapping. */
 #ifndef IMMERDINK_B200_LINEAR_H
 #define IMMERDINK_B200_LINEAR_H
 

@@ -79,3 +79,56 @@ def test_general_way_with_tensors():
             assert imd.linear_w4(x, w4, z, scale, group=32, lib=use) is z
             got.append((q, s, h, y, z))
         assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+@pytest.mark.parametrize("rows", [1, 3, 20, 77, 400])
+@pytest.mark.parametrize("skew", [0, 1])
+def test_columns_of_one_buffer(rows, skew):
+    """Inputs and outputs in columns of one buffer, side by side without a byte between them (aligned or not): the same as in
+    buffers of their own, and the columns around them stay as they were."""
+    dim, n, k = 520, 136, 264
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    raw = torch.randint(0, 256, (rows, 8192), generator=g, device="cuda", dtype=torch.uint8)
+    used = torch.zeros(rows, 8192, dtype=torch.bool, device="cuda")
+
+    def column(dtype, cols, at):
+        size = torch.empty(0, dtype=dtype).element_size()
+        used[:, at * size:(at + cols) * size] = True
+        return raw.view(dtype)[:, at:at + cols]
+
+    x, r, h = (column(BF16, dim, skew + i * dim) for i in range(3))        # bytes 0 to 6 dim
+    q = column(I8, dim, 2 * skew + 6 * dim)
+    x.normal_(generator=g), r.normal_(generator=g)
+    w = torch.randn(dim, generator=g, device="cuda").to(BF16)
+    before = raw.clone()
+    s, s2, q2, h2 = torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda"), torch.empty(rows, dim, dtype=I8, device="cuda"), torch.empty(rows, dim, dtype=BF16, device="cuda")
+    own_x, own_r = x.contiguous().clone(), r.contiguous().clone()
+    imd.norm_quantize(x, w, q, s, residual=r, residual_out=h)
+    imd.norm_quantize(own_x, w, q2, s2, residual=own_r, residual_out=h2)
+    # (a whole and a shifted row may be summed in another order: the formula within a code, and h, are the same)
+    assert torch.equal(h, h2) and bool(((s - s2).abs() <= 1e-6 * s2).all()) and int((q.int() - q2.int()).abs().max()) <= 1
+    assert torch.equal(raw[~used], before[~used]) and torch.equal(x, own_x) and torch.equal(r, own_r)
+    # 8 bits: x in one column, the output in the next
+    q, y = column(I8, k, 0), column(F32, n, (k + 4) // 4 + skew)
+    q.copy_(q2[:, :k])
+    w8, ws = torch.randint(-128, 128, (n, k), generator=g, device="cuda", dtype=torch.int32).to(I8), torch.rand(n, generator=g, device="cuda")
+    y2, used[:] = torch.empty(rows, n, device="cuda"), False
+    q, y = column(I8, k, 0), column(F32, n, (k + 4) // 4 + skew)
+    before = raw.clone()
+    imd.scaled_linear(q, w8, y, s2, ws)
+    imd.scaled_linear(q.contiguous(), w8, y2, s2, ws)
+    assert torch.equal(y, y2) and torch.equal(raw[~used], before[~used])
+    # 4 bits: the same, the output before x
+    used[:] = False
+    y, x = column(BF16, n, skew), column(BF16, k, n + skew)
+    x.copy_(own_x[:, :k])
+    w4 = torch.randint(0, 256, (n, k // 2), generator=g, device="cuda", dtype=torch.uint8)
+    scale = torch.rand(n, -(-k // 64), generator=g, device="cuda").to(BF16)
+    y2, before = torch.empty(rows, n, dtype=BF16, device="cuda"), raw.clone()
+    imd.linear_w4(x, w4, y, scale, group=64)
+    imd.linear_w4(x.contiguous(), w4, y2, scale, group=64)
+    q4 = torch.stack((w4 & 15, w4 >> 4), 2).flatten(1).double() - 8
+    size = x.double().abs() @ (q4.abs() * scale.double().repeat_interleave(64, 1)[:, :k]).t()
+    # (other kernels for shifted rows: two sums of k terms, each within k 2^-23 of their size, and two roundings to bf16)
+    assert bool(((y.double() - y2.double()).abs() <= 2 * k * 2.0 ** -23 * size + 2 * 2.0 ** -8 * y2.double().abs() + 1e-30).all())
+    assert torch.equal(raw[~used], before[~used])
