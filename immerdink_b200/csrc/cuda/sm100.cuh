@@ -9,8 +9,9 @@
 
 namespace imd {
 
-constexpr uint32_t kSpinLimit = 1u << 26;  // try_wait polls before a wait gives up
-constexpr uint32_t kLandLimit = 1u << 20;  // and before copies in flight are given up
+// An unanswered try_wait takes 1.5 us.
+constexpr uint32_t kSpinLimit = 1u << 26;  // polls before a wait gives up (100 s)
+constexpr uint32_t kLandLimit = 1u << 16;  // and before copies in flight are given up (0.1 s a slot)
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
