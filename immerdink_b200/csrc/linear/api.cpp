@@ -12,6 +12,7 @@ using i128 = __int128;
 
 constexpr int64_t kMaxExtent = INT64_C(1) << 31;  // rows, n, k, dim stay below this
 constexpr int64_t kMaxI8Depth = 131071;           // k * 128^2 < 2^31
+constexpr double kMostEps = 0x1p127;              // mean + eps stays in the range of 32 bits
 
 bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 bool is_float(int32_t t) { return t == IMD_TYPE_F32 || t == IMD_TYPE_BF16 || t == IMD_TYPE_F16; }
@@ -58,7 +59,7 @@ imd_status_t imd_norm_quantize(int64_t rows, int64_t dim, int32_t x_type, const 
                                void* residual_out, int64_t residual_out_stride, int32_t q_type,
                                void* q, int64_t q_stride, float* scale, cudaStream_t stream) {
   if (!extent_ok(rows) || !extent_ok(dim) || dim == 0 || !is_float(x_type) || !is_8bit(q_type) ||
-      !is_float(weight_type) || !(eps >= 0.0) || std::isinf(eps))
+      !is_float(weight_type) || !(eps >= 0.0 && eps <= kMostEps))
     return IMD_STATUS_INVALID_VALUE;
   if (weight_type != x_type && weight_type != IMD_TYPE_F32) return IMD_STATUS_NOT_SUPPORTED;
   if (rows == 0) return IMD_STATUS_SUCCESS;

@@ -46,7 +46,7 @@ enum { IMD_TYPE_F32 = 0, IMD_TYPE_BF16 = 1, IMD_TYPE_F16 = 2, IMD_TYPE_I8 = 3, I
  * x [rows, dim] and residual (NULL = none) in x_type (F32, BF16, F16); weight [dim] in x_type or
  * F32; q [rows, dim] in q_type (I8: Q = 127, E4M3: Q = 448); scale [rows] F32. residual_out (NULL =
  * not wanted; requires residual) receives h rounded once to x_type; it may be x or residual itself
- * (same address and stride). eps >= 0.
+ * (same address and stride). 0 <= eps <= 2^127.
  *
  * Everything between the loads and the stores is held in 32 bits: the norm sees the unrounded sum
  * h. Squares that would leave the range of 32 bits are summed again after an exact scaling by a

@@ -71,3 +71,9 @@ def test_columns_of_one_buffer_in_products(lib):
     assert lib.imd_linear_w4(*(W4 | out | dict(xs=P // 2, out=A + 127)).values()) == ALIASING
     assert lib.imd_linear_w4(*(W4 | out | dict(xs=P // 2, w=A + 256, ws=P, scale=A + 320, ss=P // 2, zeros=A + 400, zs=P)).values()) == MISALIGNED
     assert lib.imd_linear_w4(*(W4 | out | dict(xs=P // 2, zeros=A + 140, zs=P)).values()) == ALIASING
+
+
+@pytest.mark.parametrize("eps, status", [(0.0, MISALIGNED), (2.0 ** 127, MISALIGNED), (1.8e38, INVALID), (1e39, INVALID), (1e300, INVALID)])
+def test_eps_stays_in_the_range_of_32_bits(lib, eps, status):
+    """mean + eps is formed in 32 bits: an eps beyond them would turn every row to zeros."""
+    assert lib.imd_norm_quantize(*(NORM | dict(eps=eps)).values()) == status

@@ -132,3 +132,20 @@ def test_columns_of_one_buffer(rows, skew):
     # (other kernels for shifted rows: two sums of k terms, each within k 2^-23 of their size, and two roundings to bf16)
     assert bool(((y.double() - y2.double()).abs() <= 2 * k * 2.0 ** -23 * size + 2 * 2.0 ** -8 * y2.double().abs() + 1e-30).all())
     assert torch.equal(raw[~used], before[~used])
+
+
+def test_large_eps():
+    """Rows and eps at the upper end of 32 bits: the sum of squares leaves the range, mean + eps does not."""
+    rows, dim = 4, 300
+    x = torch.randn(rows, dim, device="cuda")
+    x *= torch.tensor([1.0, 1e17, 1e19, 1e30], device="cuda")[:, None]
+    w = 1 + 0.1 * torch.randn(dim, device="cuda")
+    for eps in (1e30, 1e37, 2.0 ** 127):
+        q, s = torch.empty(rows, dim, dtype=I8, device="cuda"), torch.empty(rows, device="cuda")
+        imd.norm_quantize(x, w, q, s, eps=eps)
+        y = x.double() * torch.rsqrt(x.double().square().mean(1, keepdim=True) + eps) * w.double()
+        top = y.abs().amax(1)
+        rel = ((64 + 12) / 2 + 9) * 2.0 ** -24   # a chain of at most 64 additions before the root, 9 roundings after it
+        assert bool(((s.double() - top / 127).abs() <= rel * top / 127 + 2.0 ** -149).all())
+        v = y / (top / 127)[:, None]
+        assert bool(((q.double() - v).abs() <= 0.5 + 2 * rel * v.abs() + 1e-12).all())
