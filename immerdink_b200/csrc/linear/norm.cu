@@ -3,6 +3,11 @@
 //   h = x + r;  y_j = h_j * rsqrt(mean h^2 + eps) * w_j;  a = max_j |y_j|;  scale = a / Q;
 //   q_j = round(y_j * (Q / a))                                       Q = 127 (int8), 448 (e4m3)
 //
+// The row's factor r = rsqrt(..) cancels in y_j / a. So it is split into a power of two p and m in [1, 2): the codes follow from
+// g_j = h_j p w_j, whatever r was rounded to, and the scale is max |g_j| m / Q. Q / max |g| is held in two parts, so that g_j
+// times it is rounded once: a value in the middle of two codes goes to the even one where h_j w_j is exact in 32 bits (with
+// one part and with r in the products such values went to either side).
+//
 // Bound by HBM: 2 + 2 + 2 + 1 bytes per element for 16-bit x with a residual that is written back (8191 x 8192: 78 us, 6.0
 // TB/s, 0.92 of the measured copy rate; f32 135 us, 0.99). Without a residual and for int8 bound by issue.
 // A row is read once: its values stay in registers (`E` vectors per thread) through both row
@@ -200,24 +205,43 @@ __device__ __forceinline__ void store_any(T* at, const float* f, int n) {
   if (n > 0) store_bytes<4>(reinterpret_cast<uint8_t*>(at), o, n < V ? n * static_cast<int>(sizeof(T)) : 16);
 }
 
-// What turns a row's y into codes: q = round(y * pre * inv), scale as stored.
+// r as p * m, p a power of two and m in [1, 2). An r below the normal range, an infinity and a NaN are p.
+struct Factor {
+  float p, m;
+};
+__device__ __forceinline__ Factor split(float r) {
+  const uint32_t bits = __float_as_uint(r), e = bits & 0x7F800000u;
+  if (e == 0 || e == 0x7F800000u) return {r, 1.0f};
+  return {__uint_as_float(e), __uint_as_float((bits & 0x007FFFFFu) | 0x3F800000u)};
+}
+
+// What turns a row's g into codes: q = round(g * pre * (inv + low)). `top`: the bits of the largest |g|; most = max |g| m,
+// Q times the scale.
 struct RowScale {
-  float pre, inv, scale;
+  float pre, inv, low, most;
   uint32_t keep;  // all ones, or zero for a row without a finite scale
 };
-__device__ __forceinline__ RowScale row_scale(uint32_t top, float q_max) {
-  RowScale s{1.0f, 0.0f, 0.0f, ~0u};
-  if (top >= 0x7F800000u) {
-    s.inv = s.scale = __uint_as_float(0x7FC00000u);  // a NaN or an infinity in the row
+__device__ __forceinline__ RowScale row_scale(uint32_t top, float m, bool e4m3) {
+  const float q_max = e4m3 ? 448.0f : 127.0f;
+  RowScale s{1.0f, 0.0f, 0.0f, __uint_as_float(top) * m, ~0u};
+  if (!(s.most < __uint_as_float(0x7F800000u))) {
+    s.inv = s.most = __uint_as_float(0x7FC00000u);  // a NaN or an infinity in the row
     s.keep = 0;
   } else if (top != 0) {
-    const float a = __uint_as_float(top);
-    s.scale = a / q_max;
-    if (a < 0x1p-100f) s.pre = 0x1p+100f;  // Q / a would leave the range
-    s.inv = q_max / (a * s.pre);
+    float a = __uint_as_float(top), inverse;
+    if (a < 0x1p-100f) s.pre = 0x1p+100f, a *= 0x1p+100f;  // Q / a would leave the range
+    asm("rcp.approx.f32 %0, %1;" : "=f"(inverse) : "f"(a));  // within an ulp; the second part makes up for that too
+    s.inv = inverse * q_max;
+    s.low = fmaf(-s.inv, a, q_max) * inverse;
   }
   return s;
 }
+// most / Q: the product with the rounded 1 / Q, corrected by its remainder.
+__device__ __forceinline__ float scale_of(float most, bool e4m3) {
+  const float q_max = e4m3 ? 448.0f : 127.0f, inverse = e4m3 ? 1.0f / 448.0f : 1.0f / 127.0f, s = most * inverse;
+  return fmaf(fmaf(-s, q_max, most), inverse, s);
+}
+__device__ __forceinline__ float code_value(float g, const RowScale& s) { return fmaf(g, s.inv, g * s.low); }
 
 struct Shared {
   float sums[2][32];
@@ -277,16 +301,17 @@ __global__ void __launch_bounds__(1024) k_norm_quantize_long(const __grid_consta
       ss = row_sum<false>(ss, s.sums[1]);
       r = root_down(ss / static_cast<float>(p.dim), p.eps_root, top, d.e);
     }
+    const Factor f = split(r);
     uint32_t top = 0;
-    for (int64_t j = threadIdx.x; j < p.dim; j += blockDim.x) top = max(top, magnitude(sum(j) * d.f1 * d.f2 * r * weight(j)));
-    const RowScale q = row_scale(row_max<false>(top, s.tops[1]), e4m3 ? 448.0f : 127.0f);
+    for (int64_t j = threadIdx.x; j < p.dim; j += blockDim.x) top = max(top, magnitude(sum(j) * d.f1 * d.f2 * f.p * weight(j)));
+    const RowScale q = row_scale(row_max<false>(top, s.tops[1]), f.m, e4m3);
     for (int64_t j = threadIdx.x; j < p.dim; j += blockDim.x) {
       const float h = sum(j);
       if (p.residual_out != nullptr) static_cast<T*>(p.residual_out)[row * p.residual_out_stride + j] = from_float<T>(h);
-      const float y = h * d.f1 * d.f2 * r * weight(j) * q.pre * q.inv;
+      const float y = code_value(h * d.f1 * d.f2 * f.p * weight(j) * q.pre, q);
       store_codes<1>(static_cast<uint8_t*>(p.q) + row * p.q_stride, j, &y, e4m3, q.keep);
     }
-    if (threadIdx.x == 0) p.scale[row] = q.scale;
+    if (threadIdx.x == 0) p.scale[row] = scale_of(q.most, e4m3);
   }
 }
 
@@ -350,37 +375,44 @@ __device__ __forceinline__ void finish_row(const NormArgs& p, int64_t row, int t
         for (int v = 0; v < V; ++v) h[i][v] = h[i][v] * d.f1 * d.f2;
     }
   }
+  const Factor f = split(r);
   uint32_t top = 0;
   if (same) {
 #pragma unroll
     for (int i = 0; i < E; ++i)
 #pragma unroll
-      for (int v = 0; v < V; ++v) h[i][v] = h[i][v] * r * w[i].value(v);
+      for (int v = 0; v < V; ++v) h[i][v] = h[i][v] * f.p * w[i].value(v);
   } else {
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       const int j = (i * threads + t) * V;
 #pragma unroll
       for (int v = 0; v < V; ++v)
-        if (j + v < dim) h[i][v] = h[i][v] * r * static_cast<const float*>(p.weight)[j + v];
+        if (j + v < dim) h[i][v] = h[i][v] * f.p * static_cast<const float*>(p.weight)[j + v];
     }
   }
 #pragma unroll
   for (int i = 0; i < E; ++i)
 #pragma unroll
     for (int v = 0; v < V; ++v) top = max(top, magnitude(h[i][v]));
-  const RowScale c = row_scale(row_max<WARP>(top, s.tops[1]), e4m3 ? 448.0f : 127.0f);
+  const RowScale c = row_scale(row_max<WARP>(top, s.tops[1]), f.m, e4m3);
+  if (c.pre != 1.0f) {  // rare, the same for the row
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+#pragma unroll
+      for (int v = 0; v < V; ++v) h[i][v] *= c.pre;
+  }
 #pragma unroll
   for (int i = 0; i < E; ++i) {
     const int j = (i * threads + t) * V;
     if (j < dim) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) h[i][v] = h[i][v] * c.pre * c.inv;
+      for (int v = 0; v < V; ++v) h[i][v] = code_value(h[i][v], c);
       if constexpr (ANY) store_codes_any<V>(static_cast<uint8_t*>(p.q) + row * p.q_stride + j, h[i], dim - j, e4m3, c.keep);
       else store_codes<V>(static_cast<uint8_t*>(p.q) + row * p.q_stride, j, h[i], e4m3, c.keep);
     }
   }
-  if (t == 0) p.scale[row] = c.scale;
+  if (t == 0) p.scale[row] = scale_of(c.most, e4m3);
 }
 
 // Rows in registers, one per warp or per CTA.

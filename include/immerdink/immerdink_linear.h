@@ -49,7 +49,8 @@ enum { IMD_TYPE_F32 = 0, IMD_TYPE_BF16 = 1, IMD_TYPE_F16 = 2, IMD_TYPE_I8 = 3, I
  * (same address and stride). 0 <= eps <= 2^127.
  *
  * Everything between the loads and the stores is held in 32 bits: the norm sees the unrounded sum
- * h. Squares that would leave the range of 32 bits are summed again after an exact scaling by a
+ * h. Codes are the nearest (in the middle of two: the even one) to Q y / max |y|, in which the row's root cancels: they
+ * follow from h * weight, however the root was rounded. Squares that would leave the range of 32 bits are summed again after an exact scaling by a
  * power of two. A row of zeros gives zeros and scale 0. A row whose y holds a NaN or an infinity
  * gets scale NaN (codes 0 for I8, NaN for E4M3), so that a product with it is NaN. */
 IMD_API imd_status_t imd_norm_quantize(int64_t rows, int64_t dim, int32_t x_type, const void* x,

@@ -149,3 +149,22 @@ def test_large_eps():
         assert bool(((s.double() - top / 127).abs() <= rel * top / 127 + 2.0 ** -149).all())
         v = y / (top / 127)[:, None]
         assert bool(((q.double() - v).abs() <= 0.5 + 2 * rel * v.abs() + 1e-12).all())
+
+
+@pytest.mark.parametrize("rows, dim", [(1, 4096), (70, 100), (600, 1024), (5003, 640), (5003, 2052), (900, 8192), (300, 5001), (40, 16392), (9, 40001)])
+@pytest.mark.parametrize("t, to", [(BF16, E4M3), (BF16, I8), (F16, E4M3), (F16, I8), (F32, E4M3)])
+def test_codes_are_the_nearest(rows, dim, t, to):
+    """Products g = x w of few bits: Q g / max |g| is either in the middle of two codes, which goes to the even one, or more than
+    2^-22 of itself away from it, which 32 bits tell apart (24-bit quotients are off by 2^-24). Codes have to be equal."""
+    g = torch.Generator(device="cuda").manual_seed(dim + rows)
+    x = torch.randn(rows, dim, generator=g, device="cuda").to(BF16).to(t) if t != F16 else torch.randn(rows, dim, generator=g, device="cuda").to(F16)
+    if t == BF16 and to == E4M3:
+        w = (1 + 0.2 * torch.randn(dim, generator=g, device="cuda")).to(BF16)   # g: 16 bits, middle of two codes: 5 bits; 2^-21
+    else:
+        w = torch.exp2(torch.randint(-1, 2, (dim,), generator=g, device="cuda").float()).to(t)   # g: 8 or 11 bits, middle: 5 or 8; 2^-19
+    q, s = torch.empty(rows, dim, dtype=to, device="cuda"), torch.empty(rows, device="cuda")
+    imd.norm_quantize(x, w, q, s)
+    p = x.double() * w.double()
+    v = (127.0 if to == I8 else 448.0) * p / p.abs().amax(1, keepdim=True)      # one rounding, to 53 bits
+    step = torch.ones_like(v) if to == I8 else torch.ldexp(torch.ones_like(v), (torch.frexp(v)[1] - 4).clamp(min=-9))
+    assert torch.equal(torch.round(v / step) * step, q.double())
