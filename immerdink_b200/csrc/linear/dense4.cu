@@ -15,10 +15,10 @@
 //         (rows that TMA cannot bring: x by warpgroups 2 and 3, each row's weights by the thread that unpacks it)
 //   1     thread r turns row r of the weights' next 64 k into 16-bit floats in the swizzled layout
 //   2, 3  halves of the rows of x: out += scale * accumulator, then the stores
-// Bound by what the roles' own loops take at one to three warps per scheduler: 1000 to 1150 cycles a block of 64 k with
-// groups of 128 (the MMAs of 256 rows of x need 512; a second unpacking warpgroup changes nothing), 500 more for
-// each further group in it. 28672 x 8192, g128: 140 us at 33 rows, 155 at 256; 2048 x 8192 x 8192 304 us (0.55 of the measured
-// bf16 rate), with groups of 64 440, of 32 758. Hence few and wide instructions a group: multiply-adds in pairs (316 against 304
+// Bound by what the roles' own loops take at one to three warps per scheduler. A block of 64 k takes, at 33 and at 256 rows of x,
+// 1050 and 1150 cycles with groups of 128 (the MMAs of 256 rows need 512; a second unpacking warpgroup changes nothing), 1190 and
+// 1630 with groups of 64, 1920 and 2870 with two groups of 32, whose sums bound it at 950 to 1450 cycles a group. 28672 x 8192, g128: 141
+// us at 33 rows, 154 at 256; 2048 x 8192 x 8192 304 us (0.55 of the measured bf16 rate), with groups of 64 433, of 32 762. Hence few and wide instructions a group: multiply-adds in pairs (316 against 304
 // us), eight scales in one load. A cluster of up to 8 CTAs splits K (whole groups) where the row tiles
 // alone would not fill the GPU; the parts are added through distributed shared memory in rank order.
 // Every wait is bounded, as in the 8-bit kernels.

@@ -2,8 +2,10 @@
 //
 //   out[t, n] = xs[t] ws[n] sum_k x[t, k] w[n, k]         int8: exact int32 sums; e4m3: 32-bit float sums
 //
-// Bound by the tensor pipe once both operands have a few hundred rows (int8 8192^3 333 us, 3300 T/s), by the weights'
-// bytes below (e4m3 48 x 28672 x 8192 42 us, 5.7 TB/s, 0.87 of the measured copy rate; 1 row 41 us).
+// Bound by the tensor pipe once both operands have a few hundred rows (int8 8192^3 335 to 350 us in a short run of calls, 3100 to 3300
+// T/s; 400 us, 2750 T/s, in a long one, under the power cap), by the weights' bytes below (e4m3 48 x 28672 x 8192 42 us, 5.7
+// TB/s, 0.87 of the measured copy rate; 1 row 41 us). Between, 129 to 256 rows leave one CTA on an SM, whose tiles may fill their
+// rounds badly: 256 x 28672 x 8192 has 224 of them on 148 SMs, two rounds for the work of 1.5 (62 us for 37).
 // Two kernels share the pipeline of the contraction's GEMM (TMA into a ring of 128-byte K blocks with the
 // 128-byte swizzle, one thread issuing tcgen05.mma, accumulators in tensor memory):
 //

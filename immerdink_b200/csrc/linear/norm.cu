@@ -8,8 +8,9 @@
 // times it is rounded once: a value in the middle of two codes goes to the even one where h_j w_j is exact in 32 bits (with
 // one part and with r in the products such values went to either side).
 //
-// Bound by HBM: 2 + 2 + 2 + 1 bytes per element for 16-bit x with a residual that is written back (8191 x 8192: 78 us, 6.0
-// TB/s, 0.92 of the measured copy rate; f32 135 us, 0.99). Without a residual and for int8 bound by issue.
+// Bound by HBM with a residual that is written back, 2 + 2 + 2 + 1 bytes per element of 16 bits (8191 x 8192: 79 us, 6.0
+// TB/s, 0.91 of the measured copy rate; f32 139 us, 0.95). Without a residual the bytes are 3 and 5, and instructions and the
+// two reductions' barriers bound it: 61 us (int8 codes 63, f32 78), 0.67 instructions a cycle and scheduler, 0.5 (f32 0.65) of the copy rate.
 // A row is read once: its values stay in registers (`E` vectors per thread) through both row
 // reductions, the sum of squares and the largest |y|. Short rows take one warp each, longer rows
 // one CTA; rows beyond the register capacity are read three times (twice from L2).
@@ -416,7 +417,7 @@ __device__ __forceinline__ void finish_row(const NormArgs& p, int64_t row, int t
 }
 
 // Rows in registers, one per warp or per CTA.
-// Up to 64 registers allow 1024 threads (f32 64 x 14128 with the residual: 6.2 us, by repeated passes 12.8; 4000 x 16384: 153
+// Up to 64 registers allow 1024 threads (f32 64 x 14128 with the residual: 6.6 us, by repeated passes 12.8; 4000 x 16384: 147
 // against 352).
 template <int V, int E>
 constexpr int kMostThreads = V * E <= 16 ? 1024 : 512;

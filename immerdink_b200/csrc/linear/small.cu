@@ -1,5 +1,5 @@
-// Products of operands whose rows start anywhere, with any number of rows: what the kernels that move 16-byte
-// units (stream.cu, dense8.cu, dense4.cu) cannot take.
+// Products of operands whose rows start anywhere, with few rows of x or little work (choice.hpp): more of it is quicker on
+// the tensor-core kernels (dense8.cu, dense4.cu), which then bring the rows as words too.
 //
 //   8 bits:  out[t, n] = xs[t] ws[n] sum_k x[t, k] w[n, k]
 //   4 bits:  out[t, n] = sum_g ws[n, g] sum_{k in g} x[t, k] (w[n, k] - z[n, g])

@@ -1,10 +1,10 @@
-// 4-bit products with up to 16 rows of x: the weights are streamed once.
+// 4-bit products with up to 16 rows of x in one pass over the weights; 17 to 32 rows in two where that is quicker (choice.hpp).
 //
 //   out[t, n] = sum_g ws[n, g] sum_{k in g} x[t, k] (w[n, k] - z[n, g])
 //
 // Bound by the issue and latency of the unpacking (18.7 instructions for 8 weights and lane, 11 of them the unpacking itself)
 // at 16 warps per SM, well before HBM (n k / 2 bytes): 1 row x 28672 x 8192 34 us with groups of 128 (3.6 TB/s, 0.54 of the
-// measured copy rate), 44 us with groups of 64 and zero points; 16 rows 60 and 67 us.
+// measured copy rate), 44 us with groups of 64 and zero points; 16 rows 61 and 67 us.
 //
 // A persistent CTA walks tiles of 16 MT rows of w; its eight warps take 256 k of every row (a piece) in turn. A warp has its
 // own ring of pieces that arrive by TMA, one instruction each, so the bytes in flight depend on neither registers nor

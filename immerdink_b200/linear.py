@@ -6,7 +6,7 @@
 
 Same rules as `contract`: nothing here allocates device memory, copies data or synchronises; a call
 checks the arrays on the host and enqueues kernels on the caller's stream (default: the default
-stream), so it can be captured in a CUDA graph. The caller owns every array. Arrays are PyTorch
+stream, also inside `torch.cuda.stream(s)`: pass stream=s there), so it can be captured in a CUDA graph. The caller owns every array. Arrays are PyTorch
 tensors, DLPack producers or `__cuda_array_interface__` objects; bfloat16 and float8_e4m3fn need
 one of the first two. They must be on the current device, and rows must have unit stride.
 

@@ -63,8 +63,10 @@ IMD_API imd_status_t imd_norm_quantize(int64_t rows, int64_t dim, int32_t x_type
 /* Product of two 8-bit operands with a scale per row of each.
  *
  * x [rows, k] and w [n, k], both `type` (I8 or E4M3); x_scale [rows], w_scale [n] F32; out [rows, n]
- * in out_type (F32, BF16, F16), rounded once. I8 sums are exact 32-bit integers (k <= 131071, else
- * NOT_SUPPORTED); E4M3 sums are 32-bit floats. k = 0 gives zeros. */
+ * in out_type (F32, BF16, F16). I8 sums are exact 32-bit integers (k <= 131071, else NOT_SUPPORTED);
+ * E4M3 sums are 32-bit floats, to which a tensor instruction may add its aligned terms cut instead of
+ * rounded (2^-23 of the partial sum). The sum, as a 32-bit float, times x_scale, times w_scale: each
+ * rounded in 32 bits, then to out_type. k = 0: sums of 0. */
 IMD_API imd_status_t imd_scaled_linear(int64_t rows, int64_t n, int64_t k, int32_t type,
                                        const void* x, int64_t x_stride, const void* w,
                                        int64_t w_stride, const float* x_scale,
@@ -78,7 +80,7 @@ IMD_API imd_status_t imd_scaled_linear(int64_t rows, int64_t n, int64_t k, int32
  * consecutive k, the last one possibly shorter; w_scale [n, ceil(k / group)] in scale_type (F32,
  * BF16, F16), its rows scale_stride elements apart; zeros [n, ceil(k / group)] one byte each, values
  * 0..15 (a larger byte is taken modulo 16), zeros_stride bytes apart, NULL = 8 everywhere; out
- * [rows, n] in out_type (F32 or x_type), rounded once. w - zero is exact, sums are 32-bit floats,
+ * [rows, n] in out_type (F32 or x_type), rounded once from 32 bits. w - zero is exact, sums are 32-bit floats,
  * the scale multiplies a group's sum in 32 bits. k = 0 gives zeros. */
 IMD_API imd_status_t imd_linear_w4(int64_t rows, int64_t n, int64_t k, int32_t group,
                                    int32_t x_type, const void* x, int64_t x_stride, const void* w,
