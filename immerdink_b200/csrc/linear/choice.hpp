@@ -42,7 +42,8 @@ inline int split_of(int64_t tiles, int64_t steps, const int* clusters, int ctas_
 
 // 4 bits, streamed: up to 16 rows of x in one pass over the weights. 17 to 32 take two passes where the tensor-core kernel,
 // whose time hardly depends on the rows, is slower: with groups of 32, whose sums bound it, and where its tiles leave much of
-// their last round idle; little is enough from kStreamTallN rows of w on, where a streamed tile has 32 of them.
+// their last round idle; little is enough from kStreamTallN rows of w on, where a streamed tile has 32 of them. (And with rows of x
+// that only loads bring there, such as a repeated one.)
 // (us, two passes / tensor cores, zero points: 24 x 8192 x 28672 g32 163 / 219; idle more than a third, 24 x 2048 x 2048 g128
 // 9.1 / 10.9, 24 x 4736 x 2816 g64 14 / 20; idle 14 %, 17 x 4096 x 4096 g128 16.8 / 16.1, 32 rows 20.8 / 16.4, 24 x 8192 x 8192 57
 // / 40, g64 50 / 44; many rows of w, idle a quarter, 24 x 28672 x 8192 g128 123 / 139; not idle, 24 x 18944 x 3584 g128 42 / 35.)
@@ -52,7 +53,7 @@ inline int split_of(int64_t tiles, int64_t steps, const int* clusters, int ctas_
 constexpr int64_t kStreamPassRows = 16, kStreamMostRows = 32, kStreamMostK = (INT64_C(1) << 31) - 4096;
 constexpr int64_t kStreamTallN = 64 * 148;  // two tiles of 32 rows of w for each of 148 SMs
 inline bool two_passes(const LinearArgs& a, const int* clusters) {
-  if (a.group == 32) return true;
+  if (a.group == 32 || !x4_for_tma(a)) return true;
   const int64_t tiles = (a.n + 127) / 128, unit = a.group > 64 ? a.group : 64;
   const int64_t ctas = tiles * split_of(tiles, (a.k + unit - 1) / unit, clusters, 1);
   const int64_t slots = (ctas + clusters[0] - 1) / clusters[0] * clusters[0];

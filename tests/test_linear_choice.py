@@ -89,3 +89,10 @@ def test_two_streamed_passes_only_where_they_are_quicker(lib, rows):
     for n, k in ((512, 1024), (1024, 4096), (2048, 2048), (4736, 2816), (14336, 4096), (28672, 8192), (128256, 4096)):
         for group in (32, 64, 128):
             assert w4(lib, rows, n, k, group=group) == "s"
+
+
+def test_rows_of_x_that_only_loads_bring_stay_streamed(lib):
+    """A repeated row of x: the tensor-core kernel would bring it word by word."""
+    for rows in (17, 32):
+        assert w4(lib, rows, 4096, 4096, xs=0) == "s" and w4(lib, rows, 8192, 8192, xs=4096) == "s"
+        assert w4(lib, rows, 4096, 4096, xs=0, x=A + 2) == "a"
